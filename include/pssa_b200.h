@@ -362,6 +362,42 @@ int32_t pssa_b200_gemm_xwt(pssa_b200_ctx* ctx, const float* x, const float* w, s
 int32_t pssa_b200_gemm_xwt_dev(pssa_b200_ctx* ctx, const float* x, const float* w, size_t rows, size_t n, size_t k,
                                float* out, size_t ldo, int32_t epilogue, float alpha, int32_t precision);
 
+/* ------------------------------------------------------------------ products with 4-bit weights */
+
+/* Element type of a device array that an entry point takes as `void*`. */
+typedef enum pssa_b200_dtype {
+    PSSA_B200_F32 = 0,
+    PSSA_B200_BF16 = 1,
+    PSSA_B200_F16 = 2
+} pssa_b200_dtype;
+
+/*
+ * A weight matrix [n, k] in 4 bits (no counterpart in the reference, whose weights are fp32): codes [n, k/2] bytes, the even
+ * column in a byte's low half; scales [n, G] of type `scale_dtype` and, when given, zeros [n, G] bytes in 0..15, one of each for
+ * every `group` consecutive columns of a row, G = ceil(k / group) (a last group may be shorter). The weight of a code c is
+ * (c - zero) * scale; without zeros, zero is 8. k is a multiple of 32; group is 32, 64 or a multiple of 128 (at most k rounded
+ * up to 128). Rows and groups are dense; codes start on a 16-byte boundary, scales on their type's.
+ *
+ * pssa_b200_w4_quantize_dev makes that form of w [n, k] (`dtype`, dense) by rounding to nearest even. Without zeros: scale =
+ * max|w| / 7 and c = clamp(rint(w / scale), -8, 7) + 8. With zeros: lo = min(w, 0), hi = max(w, 0) over the group, scale =
+ * (hi - lo) / 15, zero = clamp(rint(-lo / scale), 0, 15), c = clamp(rint(w / scale) + zero, 0, 15). Scales are rounded to their
+ * type (to its largest finite value where they are above it) before they are used. A group whose scale is 0 gets codes that
+ * stand for 0; a group with a NaN or an infinity gets a NaN scale, and products with it are NaN.
+ */
+int32_t pssa_b200_w4_quantize_dev(pssa_b200_ctx* ctx, const void* w, int32_t dtype, size_t n, size_t k, size_t group, uint8_t* codes,
+                                  void* scales, int32_t scale_dtype, uint8_t* zeros);
+/*
+ * Y[rows, n] = epilogue(X[rows, k] * W[n, k]^T) with W in 4 bits, for the few rows of a decode step: pssa_b200_gemm_xwt_dev's
+ * contract (epilogues and alpha included) with the weights read at a quarter of a bf16 matrix's bytes. x (row pitch ldx >= k) and
+ * out (row pitch ldo >= n) are of type `dtype`, element-aligned; sums are fp32, one rounding to `dtype` at the end. Code times
+ * input is exact for bf16 and fp16 inputs and, for fp32, good to 2^-22 of the input (it goes through three bf16 pieces, of
+ * which the smallest is dropped below the normal range); the scale is applied to each group's fp32 sum. A row's bits
+ * do not depend on the number of rows. x and out must not overlap. Only enqueues; needs no workspace.
+ */
+int32_t pssa_b200_gemv_w4_dev(pssa_b200_ctx* ctx, const void* x, int32_t dtype, size_t rows, size_t ldx, const uint8_t* codes,
+                              const void* scales, int32_t scale_dtype, const uint8_t* zeros, size_t n, size_t k, size_t group, void* out,
+                              size_t ldo, int32_t epilogue, float alpha);
+
 /* ------------------------------------------------------------------ model */
 
 /* `PSSAConfigV2` (src/pssa.rs:253-331) reduced to what the forward path reads. */
@@ -496,6 +532,71 @@ int32_t pssa_b200_sample_dev(pssa_b200_ctx* ctx, float* logits, float* probs, si
                              uint64_t* rng_state, uint32_t* ids_out, uint32_t* status_out, float* confidence_out,
                              uint32_t flags);
 
+/* ------------------------------------------------------------------ log probabilities and distillation */
+
+/* The id that stands for no token: a row without a target, an absent entry of a list. */
+#define PSSA_B200_NO_TOKEN 0xffffffffu
+/* Largest number of alternatives / of a teacher's entries for a row. */
+#define PSSA_B200_MAX_TOP 64
+#define PSSA_B200_MAX_TEACHER 256
+
+/*
+ * Log probabilities of given tokens, with rank, entropy and the best alternatives, of `rows` rows of logits (`dtype`, row pitch
+ * ld >= vocab elements, element-aligned) at a temperature T > 0. The reference scores a target's cross entropy only
+ * (src/pssa.rs:2597-2750) and reports the sampled id's probability (`raw_confidence`, src/inference.rs:526-545).
+ *   z_v = (x_v - max x) / T,  l = ln sum exp z,  logprob = z_target - l,  rank = 1 + #{v: x_v > x_target},
+ *   entropy = l - sum p_v z_v (nats),  stats = {max x, l}: what the gradient call takes back,
+ *   top_ids / top_logprobs [rows, top_n]: the top_n largest by (logit desc, id asc) in that order; PSSA_B200_NO_TOKEN and -inf
+ *   behind the last id when top_n > vocab.
+ * All DEVICE pointers: targets [rows] u32 (NULL when neither logprob nor rank is wanted; PSSA_B200_NO_TOKEN: logprob 0, rank 0;
+ * another id outside the vocabulary: logprob NaN, rank 0, and PSSA_B200_ERR_TOKEN in the context's status word), logprob, entropy
+ * [rows], stats [rows, 2], rank [rows] u32; each output may be NULL. top_n <= PSSA_B200_MAX_TOP.
+ * Logits of -inf are masked ids: probability 0, log probability -inf. A row of nothing else has logprob -inf, entropy 0, stats
+ * {-inf, 0}, rank 1. A row that holds a NaN or +inf has no distribution: its fp32 results are NaN, rank 0, top_ids
+ * PSSA_B200_NO_TOKEN. A row's bits do not depend on the other rows, but may on their number.
+ */
+int32_t pssa_b200_token_logprobs_dev(pssa_b200_ctx* ctx, const void* logits, int32_t dtype, size_t rows, size_t vocab, size_t ld,
+                                     float temperature, const uint32_t* targets, float* logprob, uint32_t* rank, float* entropy,
+                                     float* stats, size_t top_n, uint32_t* top_ids, float* top_logprobs);
+/*
+ * The gradient with respect to the logits of sum over rows of grad_logprob * logprob + grad_entropy * entropy:
+ *   grad_logits_v = (1 / T) (grad_logprob (1[v = target] - p_v) - grad_entropy p_v (ln p_v + entropy)),
+ * with stats [rows, 2] and entropy [rows] as the forward call gave them for the same logits and T. grad_logprob / grad_entropy
+ * [rows]: either may be NULL (zero); grad_logprob needs targets, grad_entropy needs entropy. grad_logits (`dtype`, row pitch
+ * ld_grad >= vocab) may be the logits themselves with the same pitch (in place), and must not overlap them otherwise. A row whose
+ * weights are both zero, or that has no token and no entropy weight, gets a zero gradient whatever its logits hold, and so does a
+ * row of masked ids only. Other ids outside the vocabulary count as no token and raise PSSA_B200_ERR_TOKEN in the status word.
+ */
+int32_t pssa_b200_token_logprobs_grad_dev(pssa_b200_ctx* ctx, const void* logits, int32_t dtype, size_t rows, size_t vocab, size_t ld,
+                                          float temperature, const uint32_t* targets, const float* stats, const float* entropy,
+                                          const float* grad_logprob, const float* grad_entropy, void* grad_logits, size_t ld_grad);
+
+/* The teacher's entries are log probabilities over the whole vocabulary; the rest of their mass belongs to the ids that are not
+ * listed. Without it the teacher is the softmax of its entries. */
+#define PSSA_B200_DISTILL_REST 1u
+/*
+ * Distillation from a teacher's best ids (no counterpart in the reference): per row the divergence of the student from the teacher
+ * and, in the same call, the gradient with respect to the student's logits. With p = softmax(x / temperature):
+ *   t = softmax(teacher / teacher_temperature) over the row's entries,  kl = sum t_i (ln t_i - ln p[id_i]);
+ *   with PSSA_B200_DISTILL_REST (teacher_temperature must be 1): t_i = exp(teacher_i), r = max(1 - sum t_i, 0), p_rest = the
+ *   sum of p over the ids that are not listed, kl = sum t_i (ln t_i - ln p[id_i]) + r (ln r - ln p_rest);
+ *   ce = -ln softmax(x)[target] (at temperature 1);
+ *   grad_logits = grad_kl * d kl / d logits + grad_ce * d ce / d logits.
+ * All DEVICE pointers: logits / grad_logits (`dtype`, pitches ld, ld_grad >= vocab; grad_logits may be NULL, or the logits
+ * themselves with the same pitch), teacher_ids u32 and teacher fp32 [rows, k] (k <= PSSA_B200_MAX_TEACHER; what
+ * pssa_b200_token_logprobs_dev gives as top_ids and top_logprobs fits), kl, ce [rows] (NULL to skip), grad_kl, grad_ce [rows]
+ * (needed with grad_logits for the losses that are to be trained; NULL: zero), targets [rows] (needed by ce and grad_ce).
+ * An id of PSSA_B200_NO_TOKEN is an absent entry or target: it counts nothing, and a row without entries has kl 0. An id that is
+ * listed twice has the sum of its entries' mass. Other ids outside the vocabulary raise PSSA_B200_ERR_TOKEN in the status word
+ * and count as absent (ce NaN). ln p is held in fp32 and is -inf below its range. Masked student logits (-inf) under a teacher's mass give kl = +inf and a finite gradient; a row of masked ids only
+ * gives kl (where the teacher has mass) and ce +inf and a zero gradient. A row with a NaN or +inf gives NaN. A row whose gradient weights are all zero
+ * gets a zero gradient whatever its logits hold.
+ */
+int32_t pssa_b200_distill_topk_dev(pssa_b200_ctx* ctx, const void* logits, int32_t dtype, size_t rows, size_t vocab, size_t ld,
+                                   float temperature, const uint32_t* teacher_ids, const float* teacher, size_t k,
+                                   float teacher_temperature, const uint32_t* targets, uint32_t flags, float* kl, float* ce,
+                                   const float* grad_kl, const float* grad_ce, void* grad_logits, size_t ld_grad);
+
 /*
  * Frozen-model scorer: the forward half of the reference's chunk forward (src/pssa.rs:2597-2750 with one loop), which
  * `pssa score` / `pssa throughput` use on a frozen model (src/evaluation.rs:205-236): logits for EVERY position, then
@@ -505,6 +606,17 @@ int32_t pssa_b200_sample_dev(pssa_b200_ctx* ctx, float* logits, float* probs, si
  */
 int32_t pssa_b200_model_score(pssa_b200_model* m, uint32_t stream, const uint64_t* ids, const uint64_t* targets, size_t n,
                               float* mean_loss, float* token_loss, float* logits_out);
+
+/*
+ * pssa_b200_model_score with what pssa_b200_token_logprobs_dev gives for every position: log probability, rank and entropy of
+ * the targets and the top_n best alternatives, at `temperature`. The carry advances like a prefill's. HOST pointers: ids [n],
+ * targets [n] (NULL when neither logprob nor rank is wanted; UINT64_MAX: a position without a target), logprob, entropy [n], rank [n]
+ * u32, top_ids u64 (UINT64_MAX behind the vocabulary's end) and top_logprobs [n, top_n]; outputs may be NULL. Non-finite logits
+ * are an error, as in the scorer; outputs then hold the positions before the pass that failed.
+ */
+int32_t pssa_b200_model_score_logprobs(pssa_b200_model* m, uint32_t stream, const uint64_t* ids, const uint64_t* targets, size_t n,
+                                       float temperature, float* logprob, uint32_t* rank, float* entropy, size_t top_n, uint64_t* top_ids,
+                                       float* top_logprobs);
 
 /*
  * Observer scratch: the reference keeps, per block, the retrieval state of the last token it processed

@@ -74,6 +74,14 @@ SIGNATURES = {
                                               C.POINTER(C.c_double)]),
     "pssa_b200_model_decode_step": (C.c_int32, [_vp, _vp, _vp, _sz, _vp, _vp]),
     "pssa_b200_sample_dev": (C.c_int32, [_vp, _vp, _vp, _sz, _sz, _vp, _vp, _vp, _vp, _vp, _vp, _vp, C.c_uint32]),
+    "pssa_b200_w4_quantize_dev": (C.c_int32, [_vp, _vp, C.c_int32, _sz, _sz, _sz, _vp, _vp, C.c_int32, _vp]),
+    "pssa_b200_gemv_w4_dev": (C.c_int32, [_vp, _vp, C.c_int32, _sz, _sz, _vp, _vp, C.c_int32, _vp, _sz, _sz, _sz, _vp, _sz, C.c_int32,
+                                          C.c_float]),
+    "pssa_b200_token_logprobs_dev": (C.c_int32, [_vp, _vp, C.c_int32, _sz, _sz, _sz, C.c_float, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _vp]),
+    "pssa_b200_token_logprobs_grad_dev": (C.c_int32, [_vp, _vp, C.c_int32, _sz, _sz, _sz, C.c_float] + [_vp] * 6 + [_sz]),
+    "pssa_b200_distill_topk_dev": (C.c_int32, [_vp, _vp, C.c_int32, _sz, _sz, _sz, C.c_float, _vp, _vp, _sz, C.c_float, _vp, C.c_uint32] +
+                                   [_vp] * 5 + [_sz]),
+    "pssa_b200_model_score_logprobs": (C.c_int32, [_vp, C.c_uint32, _vp, _vp, _sz, C.c_float, _vp, _vp, _vp, _sz, _vp, _vp]),
     "pssa_b200_model_score": (C.c_int32, [_vp, C.c_uint32, _vp, _vp, _sz, _vp, _vp, _vp]),
     "pssa_b200_model_set_observer": (C.c_int32, [_vp, C.c_int32]),
     "pssa_b200_model_get_observation": (C.c_int32, [_vp, C.c_uint32, C.c_uint32, _vp, _vp, _vp, _vp]),
@@ -92,6 +100,10 @@ MEM_HANDOVER_SELFTEST = 16
 MEM_PHASE_CLOCKS = 32
 EPI_NONE, EPI_SOFTPLUS, EPI_SIGMOID, EPI_SILU, EPI_SCALE, EPI_ADD_OUT = range(6)
 PRECISION_BF16, PRECISION_FP32_EXACT = 0, 1
+F32, BF16, F16 = range(3)
+NO_TOKEN = 0xffffffff
+MAX_TOP, MAX_TEACHER = 64, 256
+DISTILL_REST = 1
 CANCEL_FN = C.CFUNCTYPE(C.c_int32, C.c_void_p)
 EXCHANGE_FN = C.CFUNCTYPE(C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t)
 

@@ -277,4 +277,68 @@ int32_t launch_times_adapter(pssa_b200_ctx* ctx, const float* w, const float* u,
 int32_t launch_cross_entropy(pssa_b200_ctx* ctx, const float* logits, const uint32_t* targets, float* loss, size_t rows, int v);
 int32_t launch_greedy(pssa_b200_ctx* ctx, const float* logits, uint32_t* out, size_t rows, int v);
 
+// token_logprobs.cu: log probabilities of given tokens and their gradient (see pssa_b200_token_logprobs_dev)
+struct LogprobParams {
+    const void* logits;
+    int dtype;
+    size_t rows, ld;
+    int vocab;
+    float temperature;
+    const uint32_t* targets;
+    float* logprob;
+    uint32_t* rank;
+    float *entropy, *stats;
+    int top_n;
+    uint32_t* top_ids;
+    float* top_logprobs;
+    int* status;
+};
+int32_t launch_token_logprobs(pssa_b200_ctx* ctx, const LogprobParams& p);
+struct LogprobGradParams {
+    const void* logits;
+    int dtype;
+    size_t rows, ld, ld_grad;
+    int vocab;
+    float temperature;
+    const uint32_t* targets;
+    const float *stats, *entropy, *grad_logprob, *grad_entropy;
+    void* grad;
+    int* status;
+};
+int32_t launch_token_logprobs_grad(pssa_b200_ctx* ctx, const LogprobGradParams& p);
+
+// distill_topk.cu
+struct DistillParams {
+    const void* logits;
+    int dtype;
+    size_t rows, ld, ld_grad;
+    int vocab, k, rest;
+    float temperature, teacher_temperature;
+    const uint32_t *teacher_ids, *targets;
+    const float *teacher, *grad_kl, *grad_ce;
+    float *kl, *ce;
+    void* grad;
+    int* status;
+};
+int32_t launch_distill_topk(pssa_b200_ctx* ctx, const DistillParams& p);
+
+// gemv_w4.cu
+struct W4Params {
+    uint8_t* codes;
+    void* scales;
+    uint8_t* zeros;
+    int scale_dtype;
+    size_t n, k, group, groups;
+};
+int32_t launch_w4_quantize(pssa_b200_ctx* ctx, const W4Params& w, const void* src, int dtype);
+struct GemvW4Params {
+    W4Params w;  // read only
+    const void* x;
+    void* out;
+    int dtype, epilogue;
+    size_t rows, ldx, ldo;
+    float alpha;
+};
+int32_t launch_gemv_w4(pssa_b200_ctx* ctx, const GemvW4Params& p);
+
 }  // namespace pssa

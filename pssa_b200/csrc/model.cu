@@ -142,7 +142,7 @@ void pssa_b200_model_destroy(pssa_b200_model* m) {
     cudaFree(m->unembed_bf16);
     cudaFree(m->state);
     cudaFree(m->obs.q_pnc), cudaFree(m->obs.buf);
-    cudaFree(m->score.logits), cudaFree(m->score.targets), cudaFree(m->score.loss);
+    cudaFree(m->score.logits), cudaFree(m->score.targets), cudaFree(m->score.loss), cudaFree(m->score.answers);
     cudaFree(m->sampler.recent), cudaFree(m->sampler.count), cudaFree(m->sampler.rng), cudaFree(m->sampler.ids);
     cudaFree(m->sampler.status), cudaFree(m->sampler.probs), cudaFree(m->sampler.conf);
     cudaFree(m->chunks.host.off), cudaFree(m->chunks.dev.off), cudaFree(m->chunks.records), cudaFree(m->chunks.carry_in);

@@ -135,6 +135,8 @@ struct pssa_b200_model {
         uint32_t* targets = nullptr;
         float* loss = nullptr;     // [rows capacity]
         size_t tile = 0, rows = 0;
+        char* answers = nullptr;   // pssa_b200_model_score_logprobs: a pass's results
+        size_t answer_bytes = 0;
     } score;
     // observer scratch (src/pssa.rs:609-619: inf_q_pnc, inf_mem_weights, inf_m_val, inf_z_final of the last forward):
     // when enabled, every block publishes those four vectors for the last token of every lane of the last call

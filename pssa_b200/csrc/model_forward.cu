@@ -930,6 +930,34 @@ int32_t pssa_b200_model_prefill_batch_dev(pssa_b200_model* m, const uint32_t* id
     return PSSA_B200_OK;
 }
 
+// The scorers' tile of full-vocabulary logits: at most 128 MiB of the pass's rows
+static size_t score_tile(const pssa_b200_model* m, size_t window) {
+    return std::max<size_t>(1, std::min(window, ((size_t)128 << 20) / (m->v * sizeof(float))));
+}
+static int32_t score_reserve(pssa_b200_model* m, size_t window, size_t tile) {
+    pssa_b200_ctx* ctx = m->ctx;
+    auto& sc = m->score;
+    if (tile <= sc.tile && window <= sc.rows) return PSSA_B200_OK;
+    PSSA_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
+    cudaFree(sc.logits), cudaFree(sc.targets), cudaFree(sc.loss);
+    sc.logits = nullptr, sc.targets = nullptr, sc.loss = nullptr, sc.tile = 0, sc.rows = 0;
+    PSSA_CUDA(ctx, cudaMalloc((void**)&sc.logits, tile * m->v * sizeof(float)));
+    PSSA_CUDA(ctx, cudaMalloc((void**)&sc.targets, window * 4));
+    PSSA_CUDA(ctx, cudaMalloc((void**)&sc.loss, window * 4));
+    sc.tile = tile, sc.rows = window;
+    return PSSA_B200_OK;
+}
+// logits of `nr` rows of features into the scorers' tile
+static int32_t score_logits(pssa_b200_model* m, const float* feats, size_t nr) {
+    pssa_b200_ctx* ctx = m->ctx;
+    const float scale = 1.0f / std::sqrt((float)m->d);
+    if (m->precision == PSSA_B200_PRECISION_FP32_EXACT)
+        return launch_gemm_exact(ctx, feats, m->unembed, m->score.logits, nr, m->v, m->d, m->v, EPI_SCALE, scale);
+    const int32_t rc = launch_to_bf16(ctx, feats, m->ws.x_bf16, nr * m->d);
+    if (rc) return rc;
+    return launch_gemm_bf16(ctx, m->ws.x_bf16, m->unembed_bf16, m->score.logits, nullptr, nr, m->v, m->d, m->v, EPI_SCALE, scale);
+}
+
 int32_t pssa_b200_model_score(pssa_b200_model* m, uint32_t stream, const uint64_t* ids, const uint64_t* targets, size_t n, float* mean_loss,
                               float* token_loss, float* logits_out) {
     if (!m || !ids || !targets || !mean_loss) return fail(m ? m->ctx : nullptr, PSSA_B200_ERR_INVALID_ARGUMENT, "score: null argument");
@@ -941,25 +969,13 @@ int32_t pssa_b200_model_score(pssa_b200_model* m, uint32_t stream, const uint64_
         if (targets[t] >= m->v) return fail(ctx, PSSA_B200_ERR_TOKEN, "target ID %llu outside model vocabulary", (unsigned long long)targets[t]);
     }
     PSSA_CUDA(ctx, cudaSetDevice(ctx->device));
-    const size_t window = std::min(n, m->max_rows);
-    // tile of full-vocabulary logits: at most 128 MiB
-    const size_t tile = std::max<size_t>(1, std::min(window, ((size_t)128 << 20) / (m->v * sizeof(float))));
+    const size_t window = std::min(n, m->max_rows), tile = score_tile(m, window);
     auto& sc = m->score;
-    if (tile > sc.tile || window > sc.rows) {
-        PSSA_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
-        cudaFree(sc.logits), cudaFree(sc.targets), cudaFree(sc.loss);
-        sc = pssa_b200_model::Score{};
-        PSSA_CUDA(ctx, cudaMalloc((void**)&sc.logits, tile * m->v * sizeof(float)));
-        PSSA_CUDA(ctx, cudaMalloc((void**)&sc.targets, window * 4));
-        PSSA_CUDA(ctx, cudaMalloc((void**)&sc.loss, window * 4));
-        sc.tile = tile, sc.rows = window;
-    }
-    const bool exact = m->precision == PSSA_B200_PRECISION_FP32_EXACT;
-    const float scale = 1.0f / std::sqrt((float)m->d);
+    int32_t rc = score_reserve(m, window, tile);
+    if (rc) return rc;
     std::vector<uint32_t> h_ids(window), h_tgt(window);
     std::vector<float> h_loss(window);
     double total = 0.0;
-    int32_t rc;
     cudaStream_t st = ctx->stream;
     for (size_t t0 = 0; t0 < n; t0 += window) {
         const size_t rows = std::min(window, n - t0);
@@ -973,12 +989,7 @@ int32_t pssa_b200_model_score(pssa_b200_model* m, uint32_t stream, const uint64_
         if ((rc = forward_rows(m, rows, 1, ws.host, &off, &len, &feats))) return rc;
         for (size_t r0 = 0; r0 < rows; r0 += tile) {
             const size_t nr = std::min(tile, rows - r0);
-            if (exact) {
-                if ((rc = launch_gemm_exact(ctx, feats + r0 * m->d, m->unembed, sc.logits, nr, m->v, m->d, m->v, EPI_SCALE, scale))) return rc;
-            } else {
-                if ((rc = launch_to_bf16(ctx, feats + r0 * m->d, ws.x_bf16, nr * m->d))) return rc;
-                if ((rc = launch_gemm_bf16(ctx, ws.x_bf16, m->unembed_bf16, sc.logits, nullptr, nr, m->v, m->d, m->v, EPI_SCALE, scale))) return rc;
-            }
+            if ((rc = score_logits(m, feats + r0 * m->d, nr))) return rc;
             if ((rc = launch_cross_entropy(ctx, sc.logits, sc.targets + r0, sc.loss + r0, nr, (int)m->v))) return rc;
             if (logits_out)
                 PSSA_CUDA(ctx, cudaMemcpyAsync(logits_out + (t0 + r0) * m->v, sc.logits, nr * m->v * sizeof(float), cudaMemcpyDeviceToHost, st));
@@ -997,6 +1008,94 @@ int32_t pssa_b200_model_score(pssa_b200_model* m, uint32_t stream, const uint64_
     }
     *mean_loss = (float)(total / (double)n);
     return PSSA_B200_OK;
+}
+
+// pssa_b200_model_score's passes with the log probabilities' kernel in place of the cross entropy's
+static int32_t score_answers(pssa_b200_model* m, uint32_t stream, const uint64_t* ids, const uint64_t* targets, size_t n, float temperature,
+                             float* logprob, uint32_t* rank, float* entropy, size_t top_n, uint64_t* top_ids, float* top_logprobs) {
+    pssa_b200_ctx* ctx = m->ctx;
+    const size_t window = std::min(n, m->max_rows), tile = score_tile(m, window);
+    auto& sc = m->score;
+    int32_t rc = score_reserve(m, window, tile);
+    if (rc) return rc;
+    // a pass's results, one array after another: log probability, entropy, rank, alternatives' ids, their log probabilities
+    const size_t words = window * (3 + 2 * top_n);
+    if (words * 4 > sc.answer_bytes) {
+        PSSA_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
+        cudaFree(sc.answers);
+        sc.answers = nullptr, sc.answer_bytes = 0;
+        PSSA_CUDA(ctx, cudaMalloc((void**)&sc.answers, words * 4));
+        sc.answer_bytes = words * 4;
+    }
+    std::vector<uint32_t> h_ids(window), h_tgt(window, PSSA_B200_NO_TOKEN), back(words);
+    for (size_t t0 = 0; t0 < n; t0 += window) {
+        const size_t rows = std::min(window, n - t0);
+        h_ids.resize(rows), h_tgt.resize(rows);
+        for (size_t t = 0; t < rows; ++t) {
+            h_ids[t] = (uint32_t)ids[t0 + t];
+            if (targets) h_tgt[t] = targets[t0 + t] == UINT64_MAX ? PSSA_B200_NO_TOKEN : (uint32_t)targets[t0 + t];
+        }
+        if ((rc = ensure_workspace(m, rows, 1))) return rc;
+        const uint32_t off = 0, len = (uint32_t)rows;
+        if ((rc = send_description(m, h_ids, {off}, {len}, {stream}, {}, {}, {}, &h_tgt, sc.targets))) return rc;
+        float* feats = nullptr;
+        if ((rc = forward_rows(m, rows, 1, m->ws.host, &off, &len, &feats))) return rc;
+        float* lp = reinterpret_cast<float*>(sc.answers);
+        float* ent = lp + rows;
+        uint32_t* rk = reinterpret_cast<uint32_t*>(ent + rows);
+        uint32_t* tid = rk + rows;
+        float* tlp = reinterpret_cast<float*>(tid + rows * top_n);
+        for (size_t r0 = 0; r0 < rows; r0 += tile) {
+            const size_t nr = std::min(tile, rows - r0);
+            if ((rc = score_logits(m, feats + r0 * m->d, nr))) return rc;
+            LogprobParams p{};
+            p.logits = sc.logits, p.dtype = PSSA_B200_F32, p.rows = nr, p.ld = m->v, p.vocab = (int)m->v, p.temperature = temperature;
+            p.targets = sc.targets + r0, p.logprob = lp + r0, p.rank = rk + r0, p.entropy = ent + r0, p.top_n = (int)top_n;
+            p.top_ids = top_n ? tid + r0 * top_n : nullptr, p.top_logprobs = top_n ? tlp + r0 * top_n : nullptr, p.status = ctx->status_dev;
+            if ((rc = launch_token_logprobs(ctx, p))) return rc;
+        }
+        PSSA_CUDA(ctx, cudaMemcpyAsync(back.data(), sc.answers, rows * (3 + 2 * top_n) * 4, cudaMemcpyDeviceToHost, ctx->stream));
+        PSSA_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
+        const float* b_lp = reinterpret_cast<const float*>(back.data());
+        const uint32_t *b_rk = back.data() + 2 * rows, *b_ids = b_rk + rows;
+        const float* b_tlp = reinterpret_cast<const float*>(b_ids + rows * top_n);
+        for (size_t t = 0; t < rows; ++t)
+            if (!std::isfinite(b_lp[rows + t])) return fail(ctx, PSSA_B200_ERR_INVALID_ARGUMENT, "model emitted non-finite logits at token %zu", t0 + t);
+        if (logprob) std::copy(b_lp, b_lp + rows, logprob + t0);
+        if (entropy) std::copy(b_lp + rows, b_lp + 2 * rows, entropy + t0);
+        if (rank) std::copy(b_rk, b_rk + rows, rank + t0);
+        for (size_t i = 0; i < rows * top_n; ++i) {
+            top_ids[t0 * top_n + i] = b_ids[i] == PSSA_B200_NO_TOKEN ? UINT64_MAX : b_ids[i];
+            top_logprobs[t0 * top_n + i] = b_tlp[i];
+        }
+    }
+    return PSSA_B200_OK;
+}
+
+int32_t pssa_b200_model_score_logprobs(pssa_b200_model* m, uint32_t stream, const uint64_t* ids, const uint64_t* targets, size_t n, float temperature,
+                                       float* logprob, uint32_t* rank, float* entropy, size_t top_n, uint64_t* top_ids, float* top_logprobs) {
+    if (!m || !ids) return fail(m ? m->ctx : nullptr, PSSA_B200_ERR_INVALID_ARGUMENT, "score: null argument");
+    pssa_b200_ctx* ctx = m->ctx;
+    if (n == 0) return fail(ctx, PSSA_B200_ERR_INVALID_ARGUMENT, "score requires at least one token");
+    if (stream >= m->max_streams) return fail(ctx, PSSA_B200_ERR_INVALID_ARGUMENT, "stream %u outside %u streams", stream, m->max_streams);
+    if ((logprob || rank) && !targets) return fail(ctx, PSSA_B200_ERR_INVALID_ARGUMENT, "score: log probability and rank need targets");
+    if ((top_n != 0) != (top_ids != nullptr) || (top_n != 0) != (top_logprobs != nullptr))
+        return fail(ctx, PSSA_B200_ERR_INVALID_ARGUMENT, "score: alternatives need top_n, top_ids and top_logprobs, all or none");
+    if (top_n > PSSA_B200_MAX_TOP) return fail(ctx, PSSA_B200_ERR_UNSUPPORTED, "score: %zu alternatives are more than %d", top_n, PSSA_B200_MAX_TOP);
+    if (!logprob && !rank && !entropy && top_n == 0) return fail(ctx, PSSA_B200_ERR_INVALID_ARGUMENT, "score: no output is asked for");
+    if (!(temperature > 0.0f) || !std::isfinite(temperature) || !std::isfinite(1.4427f / temperature))
+        return fail(ctx, PSSA_B200_ERR_INVALID_ARGUMENT, "score: temperature %g is not a positive finite number", (double)temperature);
+    for (size_t t = 0; t < n; ++t) {
+        if (ids[t] >= m->v) return fail(ctx, PSSA_B200_ERR_TOKEN, "token ID %llu outside model vocabulary", (unsigned long long)ids[t]);
+        if (targets && targets[t] >= m->v && targets[t] != UINT64_MAX)
+            return fail(ctx, PSSA_B200_ERR_TOKEN, "target ID %llu outside model vocabulary", (unsigned long long)targets[t]);
+    }
+    PSSA_CUDA(ctx, cudaSetDevice(ctx->device));
+    try {
+        return score_answers(m, stream, ids, targets, n, temperature, logprob, rank, entropy, top_n, top_ids, top_logprobs);
+    } catch (const std::bad_alloc&) {
+        return fail(ctx, PSSA_B200_ERR_INVALID_ARGUMENT, "score: out of host memory");
+    }
 }
 
 int32_t pssa_b200_model_set_observer(pssa_b200_model* m, int32_t enabled) {

@@ -32,6 +32,19 @@ def _host(a, name, shape=None):
     return a
 
 
+_DTYPES = {"float32": N.F32, "bfloat16": N.BF16, "float16": N.F16}
+
+
+def _dtype(x, given, name):
+    """The element type of a device buffer: of the tensor, or the one named ("float32", "bfloat16", "float16") for a raw pointer."""
+    own = getattr(x, "dtype", None)
+    key = str(own).removeprefix("torch.") if own is not None else given
+    if key not in _DTYPES or (given is not None and given != key):
+        raise TypeError(f"{name} must be float32, bfloat16 or float16 (name the type of a raw pointer): got {key}" +
+                        (f", {given} asked for" if own is not None and given is not None else ""))
+    return _DTYPES[key]
+
+
 class B200Dispatch:
     """One context on one B200 (`GpuDispatch::B200`)."""
 
@@ -265,6 +278,53 @@ class B200Dispatch:
                                                    _ptr(recent_count), _ptr(rng_state), _ptr(ids_out), _ptr(status_out),
                                                    _ptr(confidence_out),
                                                    N.SAMPLE_EXACT if exact else 0))
+
+    # ---- log probabilities of given tokens, distillation (device pointers)
+    def token_logprobs_dev(self, logits, rows, vocab, targets=None, logprob=None, rank=None, entropy=None, stats=None, top_n=0,
+                           top_ids=None, top_logprobs=None, temperature=1.0, ld=None, dtype=None):
+        """Log probability and rank of each row's target, entropy and the `top_n` best alternatives; only enqueues. `stats`
+        [rows, 2] is what the gradient call takes back. `dtype` names the logits' type where they are a raw pointer. See
+        pssa_b200_token_logprobs_dev in include/pssa_b200.h for masked rows and rows without a target."""
+        self._check(self._lib.pssa_b200_token_logprobs_dev(
+            self._h, _ptr(logits), _dtype(logits, dtype, "logits"), rows, vocab, vocab if ld is None else ld, temperature, _ptr(targets),
+            _ptr(logprob), _ptr(rank), _ptr(entropy), _ptr(stats), top_n, _ptr(top_ids), _ptr(top_logprobs)))
+
+    def token_logprobs_grad_dev(self, logits, rows, vocab, targets, stats, grad_logits, grad_logprob=None, entropy=None,
+                                grad_entropy=None, temperature=1.0, ld=None, ld_grad=None, dtype=None):
+        """Gradient with respect to the logits of sum(grad_logprob * logprob + grad_entropy * entropy), with `stats` and `entropy`
+        of the forward call; `grad_logits` has the logits' type and may be the logits themselves."""
+        if _dtype(grad_logits, dtype, "grad_logits") != _dtype(logits, dtype, "logits"):
+            raise TypeError("grad_logits must have the type of the logits")
+        self._check(self._lib.pssa_b200_token_logprobs_grad_dev(
+            self._h, _ptr(logits), _dtype(logits, dtype, "logits"), rows, vocab, vocab if ld is None else ld, temperature, _ptr(targets),
+            _ptr(stats), _ptr(entropy), _ptr(grad_logprob), _ptr(grad_entropy), _ptr(grad_logits), vocab if ld_grad is None else ld_grad))
+
+    def distill_topk_dev(self, logits, rows, vocab, teacher_ids, teacher, k, kl=None, grad_kl=None, targets=None, ce=None, grad_ce=None,
+                         grad_logits=None, temperature=1.0, teacher_temperature=1.0, rest=False, ld=None, ld_grad=None, dtype=None):
+        """Divergence of the student from a teacher's `k` best ids (and a target's cross entropy) and, with `grad_logits`, the
+        gradient of sum(grad_kl * kl + grad_ce * ce) in the same call. `teacher`: logits, or log probabilities whose missing mass
+        belongs to all other ids (`rest=True`). See pssa_b200_distill_topk_dev in include/pssa_b200.h."""
+        if grad_logits is not None and _dtype(grad_logits, dtype, "grad_logits") != _dtype(logits, dtype, "logits"):
+            raise TypeError("grad_logits must have the type of the logits")
+        self._check(self._lib.pssa_b200_distill_topk_dev(
+            self._h, _ptr(logits), _dtype(logits, dtype, "logits"), rows, vocab, vocab if ld is None else ld, temperature,
+            _ptr(teacher_ids), _ptr(teacher), k, teacher_temperature, _ptr(targets), N.DISTILL_REST if rest else 0, _ptr(kl), _ptr(ce),
+            _ptr(grad_kl), _ptr(grad_ce), _ptr(grad_logits), vocab if ld_grad is None else ld_grad))
+
+    # ---- products with 4-bit weights (device pointers)
+    def w4_quantize_dev(self, w, n, k, group, codes, scales, zeros=None, dtype=None, scale_dtype=None):
+        """The matrix w [n, k] as 4-bit codes [n, k/2] with a scale (and, with `zeros`, a zero) for each `group` of columns."""
+        self._check(self._lib.pssa_b200_w4_quantize_dev(self._h, _ptr(w), _dtype(w, dtype, "w"), n, k, group, _ptr(codes), _ptr(scales),
+                                                        _dtype(scales, scale_dtype, "scales"), _ptr(zeros)))
+
+    def gemv_w4_dev(self, x, rows, codes, scales, zeros, n, k, group, out, ldx=None, ldo=None, epilogue=N.EPI_NONE, alpha=1.0,
+                    dtype=None, scale_dtype=None):
+        """out[rows, n] = epilogue(x[rows, k] * W[n, k]^T) with W in 4 bits, for the few rows of a decode step; only enqueues."""
+        if _dtype(out, dtype, "out") != _dtype(x, dtype, "x"):
+            raise TypeError("out must have the type of x")
+        self._check(self._lib.pssa_b200_gemv_w4_dev(
+            self._h, _ptr(x), _dtype(x, dtype, "x"), rows, k if ldx is None else ldx, _ptr(codes), _ptr(scales),
+            _dtype(scales, scale_dtype, "scales"), _ptr(zeros), n, k, group, _ptr(out), n if ldo is None else ldo, epilogue, alpha))
 
     # ---- bank write / plastic fast weights (device pointers)
     def bank_insert_protected_dev(self, keys, norm_sq, values, confidence, last_seen_step, meta, capacity, d_key, d_val,

@@ -247,6 +247,23 @@ class PSSAModel:
                                                         _ptr(logits)))
         return (float(mean.value), per, logits) if want_logits else (float(mean.value), per)
 
+    def score_logprobs(self, ids, targets=None, top=0, temperature=1.0, stream=0):
+        """What `score` sees of every position of a frozen model, in full: a dict of `logprob` and `rank` (1 = the best id) of the
+        targets (None without `targets`; a target of -1 stands for none: log probability 0, rank 0), `entropy`, and the `top` best
+        alternatives as `top_ids` (int64, -1 behind the vocabulary's end) and `top_logprobs` [n, top]."""
+        ids = np.ascontiguousarray(ids, np.uint64)
+        out = dict(logprob=None, rank=None, entropy=np.empty(ids.size, np.float32), top_ids=np.empty((ids.size, top), np.int64),
+                   top_logprobs=np.empty((ids.size, top), np.float32))
+        if targets is not None:
+            targets = np.ascontiguousarray(np.asarray(targets).astype(np.int64)).view(np.uint64)
+            if targets.shape != ids.shape:
+                raise ValueError(f"targets have shape {targets.shape}, expected {ids.shape}")
+            out["logprob"], out["rank"] = np.empty(ids.size, np.float32), np.empty(ids.size, np.uint32)
+        self.gpu._check(self._lib.pssa_b200_model_score_logprobs(
+            self._h, stream, _ptr(ids), _ptr(targets), ids.size, temperature, _ptr(out["logprob"]), _ptr(out["rank"]),
+            _ptr(out["entropy"]), top, _ptr(out["top_ids"]) if top else None, _ptr(out["top_logprobs"]) if top else None))
+        return out
+
     def set_observer(self, enabled=True):
         """Publish each block's retrieval scratch of the last token of every lane (src/pssa.rs:609-619)."""
         self.gpu._check(self._lib.pssa_b200_model_set_observer(self._h, 1 if enabled else 0))

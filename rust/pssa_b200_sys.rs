@@ -29,6 +29,15 @@ pub const PSSA_B200_MEM_NO_FUSED: u32 = 8;
 pub const PSSA_B200_MEM_HANDOVER_SELFTEST: u32 = 16;
 pub const PSSA_B200_MEM_PHASE_CLOCKS: u32 = 32;
 pub const PSSA_B200_SAMPLE_EXACT: u32 = 1;
+pub const PSSA_B200_DISTILL_REST: u32 = 1;
+pub const PSSA_B200_NO_TOKEN: u32 = 0xffff_ffff;
+pub const PSSA_B200_MAX_TOP: usize = 64;
+pub const PSSA_B200_MAX_TEACHER: usize = 256;
+
+/// `pssa_b200_dtype`
+pub const PSSA_B200_F32: i32 = 0;
+pub const PSSA_B200_BF16: i32 = 1;
+pub const PSSA_B200_F16: i32 = 2;
 
 /// `pssa_b200_epilogue`
 pub const PSSA_B200_EPI_NONE: i32 = 0;
@@ -440,6 +449,36 @@ extern "C" {
         alpha: f32,
         precision: i32,
     ) -> i32;
+    pub fn pssa_b200_w4_quantize_dev(
+        ctx: *mut pssa_b200_ctx,
+        w: *const c_void,
+        dtype: i32,
+        n: usize,
+        k: usize,
+        group: usize,
+        codes: *mut u8,
+        scales: *mut c_void,
+        scale_dtype: i32,
+        zeros: *mut u8,
+    ) -> i32;
+    pub fn pssa_b200_gemv_w4_dev(
+        ctx: *mut pssa_b200_ctx,
+        x: *const c_void,
+        dtype: i32,
+        rows: usize,
+        ldx: usize,
+        codes: *const u8,
+        scales: *const c_void,
+        scale_dtype: i32,
+        zeros: *const u8,
+        n: usize,
+        k: usize,
+        group: usize,
+        out: *mut c_void,
+        ldo: usize,
+        epilogue: i32,
+        alpha: f32,
+    ) -> i32;
     pub fn pssa_b200_model_create(
         ctx: *mut pssa_b200_ctx,
         cfg: *const pssa_b200_config,
@@ -539,6 +578,60 @@ extern "C" {
         confidence_out: *mut f32,
         flags: u32,
     ) -> i32;
+    pub fn pssa_b200_token_logprobs_dev(
+        ctx: *mut pssa_b200_ctx,
+        logits: *const c_void,
+        dtype: i32,
+        rows: usize,
+        vocab: usize,
+        ld: usize,
+        temperature: f32,
+        targets: *const u32,
+        logprob: *mut f32,
+        rank: *mut u32,
+        entropy: *mut f32,
+        stats: *mut f32,
+        top_n: usize,
+        top_ids: *mut u32,
+        top_logprobs: *mut f32,
+    ) -> i32;
+    pub fn pssa_b200_token_logprobs_grad_dev(
+        ctx: *mut pssa_b200_ctx,
+        logits: *const c_void,
+        dtype: i32,
+        rows: usize,
+        vocab: usize,
+        ld: usize,
+        temperature: f32,
+        targets: *const u32,
+        stats: *const f32,
+        entropy: *const f32,
+        grad_logprob: *const f32,
+        grad_entropy: *const f32,
+        grad_logits: *mut c_void,
+        ld_grad: usize,
+    ) -> i32;
+    pub fn pssa_b200_distill_topk_dev(
+        ctx: *mut pssa_b200_ctx,
+        logits: *const c_void,
+        dtype: i32,
+        rows: usize,
+        vocab: usize,
+        ld: usize,
+        temperature: f32,
+        teacher_ids: *const u32,
+        teacher: *const f32,
+        k: usize,
+        teacher_temperature: f32,
+        targets: *const u32,
+        flags: u32,
+        kl: *mut f32,
+        ce: *mut f32,
+        grad_kl: *const f32,
+        grad_ce: *const f32,
+        grad_logits: *mut c_void,
+        ld_grad: usize,
+    ) -> i32;
     pub fn pssa_b200_model_score(
         m: *mut pssa_b200_model,
         stream: u32,
@@ -548,6 +641,20 @@ extern "C" {
         mean_loss: *mut f32,
         token_loss: *mut f32,
         logits_out: *mut f32,
+    ) -> i32;
+    pub fn pssa_b200_model_score_logprobs(
+        m: *mut pssa_b200_model,
+        stream: u32,
+        ids: *const u64,
+        targets: *const u64,
+        n: usize,
+        temperature: f32,
+        logprob: *mut f32,
+        rank: *mut u32,
+        entropy: *mut f32,
+        top_n: usize,
+        top_ids: *mut u64,
+        top_logprobs: *mut f32,
     ) -> i32;
     pub fn pssa_b200_model_set_observer(m: *mut pssa_b200_model, enabled: i32) -> i32;
     pub fn pssa_b200_model_get_observation(
