@@ -1,5 +1,10 @@
 // Products of a few rows with a matrix in 4 bits, and quantisation to that form (see pssa_b200_gemv_w4_dev).
 // One warp to a weight row, or to a group that is quantised.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+#include <type_traits>
+
 #include "device_math.cuh"
 #include "element.cuh"
 #include "kernels.hpp"
@@ -9,30 +14,293 @@ namespace {
 
 constexpr int kThreads = 256;
 
+// ---- product
+//
+// out[r, n] = sum over groups of scale * sum over the group's columns of (code - zero) * x. Code minus zero is a small whole number, exact in
+// bf16 and fp16, so the inner sums go through mma.m16n8k16 with 16 weight rows as A, the inputs' rows as the 8 columns of B and fp32
+// accumulators, and only a group's sum meets the scale. An fp32 input is three columns, its bits cut into three bf16 numbers that add up to it.
+//
+// A chunk is 128 columns. Lane (g, t) of a warp (g = lane / 4, t = lane % 4) loads 16 bytes, 32 codes, of rows g and g + 8, so that a row's chunk
+// is 64 bytes in a row. Which columns the four lanes of a row multiply at a time is free as long as A and B agree, but all of one product have
+// to be of one group: as they lie for groups of 128 and more, after one exchange between lanes two apart for 64, after a 4 x 4
+// transposition for 32. `place` says where a run of 8 columns ends up. A word's 8 codes become 4 registers of two columns 4 apart, by a mask and the bits
+// of 128 (fp16: 1024) that put a code into a mantissa; x is staged with its runs in that order.
+constexpr int kWarps = kThreads / 32;
+constexpr int kChunk = 128;
+
+struct W4Split {
+    int chunks;      // of 128 columns
+    int per_cta;     // of them to a CTA of the cluster, which splits the columns
+    int stage;       // of them in shared memory at a time
+    int k_warps;     // warps of a CTA that share weight rows and split the columns
+    int slice;       // input rows of a CTA
+    int vec;         // x starts and steps on 16 bytes
+};
+
 template <typename T>
-__global__ void __launch_bounds__(kThreads) gemv_w4_kernel(GemvW4Params p) {
-    const size_t n = ((size_t)blockIdx.x * kThreads + threadIdx.x) >> 5;
-    const int lane = threadIdx.x & 31;
-    if (n >= p.w.n) return;
-    for (size_t r = 0; r < p.rows; ++r) {
-        const T* x = static_cast<const T*>(p.x) + r * p.ldx;
-        float acc = 0.0f;
-        for (size_t g = 0; g < p.w.groups; ++g) {
-            const int zero = p.w.zeros ? p.w.zeros[n * p.w.groups + g] : 8;
-            float part = 0.0f;
-            for (size_t k = g * p.w.group + lane; k < min((g + 1) * p.w.group, p.w.k); k += 32) {
-                const int c = p.w.codes[(n * p.w.k + k) >> 1] >> (k & 1) * 4 & 15;
-                part = fmaf((float)(c - zero), to_f32(x[k]), part);
+struct Mma {  // fp32 inputs: three bf16 pieces
+    static constexpr int pieces = 3;
+    static constexpr uint32_t magic = 0x43004300u;
+};
+template <>
+struct Mma<__nv_bfloat16> {
+    static constexpr int pieces = 1;
+    static constexpr uint32_t magic = 0x43004300u;
+};
+template <>
+struct Mma<__half> {
+    static constexpr int pieces = 1;
+    static constexpr uint32_t magic = 0x64006400u;
+};
+
+template <typename T>
+__device__ __forceinline__ uint32_t minus2(uint32_t a, uint32_t b) {
+    if constexpr (std::is_same_v<T, __half>) {
+        const __half2 r = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+        return *reinterpret_cast<const uint32_t*>(&r);
+    } else {
+        const __nv_bfloat162 r = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+        return *reinterpret_cast<const uint32_t*>(&r);
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    if constexpr (std::is_same_v<T, __half>)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// word and lane that a chunk's run q of 8 columns ends up in
+template <int MODE>
+__device__ __forceinline__ void place(int q, int* word, int* t) {
+    if (MODE == 0)
+        *t = q >> 2, *word = q & 3;
+    else if (MODE == 2)
+        *word = q >> 2, *t = q & 3;
+    else
+        *word = (q & 1) + 2 * (q >> 3), *t = (q >> 2 & 1) + 2 * (q >> 1 & 1);
+}
+
+__device__ __forceinline__ void swap_words(uint32_t& lo, uint32_t& hi, bool upper, int mask) {
+    const uint32_t got = __shfl_xor_sync(0xffffffffu, upper ? lo : hi, mask);
+    if (upper)
+        lo = got;
+    else
+        hi = got;
+}
+template <int MODE>
+__device__ __forceinline__ void by_group(int t, uint4& w) {
+    if (MODE == 0) return;
+    if (MODE == 2) {
+        swap_words(w.x, w.y, t & 1, 1);
+        swap_words(w.z, w.w, t & 1, 1);
+    }
+    swap_words(w.x, w.z, t & 2, 2);
+    swap_words(w.y, w.w, t & 2, 2);
+}
+
+__device__ __forceinline__ uint4 load_codes(const uint8_t* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
+// 8 inputs of one run as 16-bit numbers in the order of the codes' registers: columns (0, 4), (1, 5), (2, 6), (3, 7)
+__device__ __forceinline__ uint4 interleave(uint4 v) {
+    return make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
+}
+
+// columns [8 run, 8 run + 8) of an input row into place `at` (and, for fp32, the two after it in steps of `step`)
+template <typename T>
+__device__ __forceinline__ void stage_run(const T* x, size_t col, bool in, int vec, uint4* at, int step) {
+    if constexpr (std::is_same_v<T, float>) {
+        uint32_t u[8] = {};
+        if (in) {
+            if (vec) {
+                const uint4 a = *reinterpret_cast<const uint4*>(x + col), b = *reinterpret_cast<const uint4*>(x + col + 4);
+                u[0] = a.x, u[1] = a.y, u[2] = a.z, u[3] = a.w, u[4] = b.x, u[5] = b.y, u[6] = b.z, u[7] = b.w;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) u[j] = __float_as_uint(x[col + j]);
             }
-            acc = fmaf(part, load_f32(p.w.scales, p.w.scale_dtype, n * p.w.groups + g), acc);
         }
 #pragma unroll
-        for (int m = 16; m > 0; m >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, m);
-        if (lane == 0) {
-            T* out = static_cast<T*>(p.out) + r * p.ldo + n;
-            *out = from_f32<T>(apply_epilogue(p.epilogue, acc, p.alpha, p.epilogue == EPI_ADD_OUT ? to_f32(*out) : 0.0f));
+        for (int piece = 0; piece < 3; ++piece) {
+            uint32_t o[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[j] = __byte_perm(u[j], u[j + 4], 0x7632);  // the upper halves: cut, not rounded
+            at[piece * step] = make_uint4(o[0], o[1], o[2], o[3]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) u[j] = __float_as_uint(__uint_as_float(u[j]) - __uint_as_float(u[j] & 0xffff0000u));
+        }
+    } else {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (in) {
+            if (vec) {
+                v = *reinterpret_cast<const uint4*>(x + col);
+            } else {
+                const uint16_t* h = reinterpret_cast<const uint16_t*>(x + col);
+                v = make_uint4(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16, h[4] | (uint32_t)h[5] << 16, h[6] | (uint32_t)h[7] << 16);
+            }
+        }
+        *at = interleave(v);
+    }
+}
+
+// MODE 0: groups of 128 and more, 1: of 64, 2: of 32.
+// A CTA: kWarps / k_warps warps side by side over weight rows, each with MT times 16 of them, times k_warps over the columns' chunks; up to NT times 8
+// columns of B. The CTAs of a cluster split the columns further; the first of them joins their sums. Sums are joined in a fixed order.
+template <typename T, int NT, int MT, int MODE>
+__global__ void __launch_bounds__(kThreads, 2) gemv_w4_kernel(GemvW4Params p, W4Split sp) {
+    extern __shared__ uint4 s_x[];
+    constexpr int P = Mma<T>::pieces;
+    constexpr uint32_t kMagic = Mma<T>::magic;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int wk = warp % sp.k_warps, wm = warp / sp.k_warps, m_warps = kWarps / sp.k_warps;
+    const int cta_rows = m_warps * MT * 16;
+    const size_t n0 = (size_t)blockIdx.y * cta_rows, r0 = (size_t)blockIdx.z * sp.slice;
+    const int in_rows = (int)min((size_t)sp.slice, p.rows - r0), cols = in_rows * P;
+    const int c0 = min((int)blockIdx.x * sp.per_cta, sp.chunks), c1 = min(c0 + sp.per_cta, sp.chunks);
+    const size_t row_bytes = p.w.k >> 1;
+    const int k = (int)p.w.k;
+
+    // this lane's rows are n_lane + 8 m
+    const size_t n_lane = n0 + (size_t)wm * MT * 16 + g;
+    const int left = n_lane < p.w.n ? (int)min(p.w.n - n_lane, (size_t)MT * 16) : 0;
+    const uint8_t* codes = p.w.codes + (left ? n_lane : 0) * row_bytes + 16 * t;
+    const size_t scale0 = (left ? n_lane : 0) * p.w.groups;
+    auto fetch = [&](int chunk, uint4 (&w)[2 * MT]) {
+        const bool in = chunk < c1 && chunk * kChunk + 32 * t < k;
+#pragma unroll
+        for (int m = 0; m < 2 * MT; ++m) w[m] = in && 8 * m < left ? load_codes(codes + m * 8 * row_bytes + (size_t)chunk * (kChunk / 2)) : make_uint4(0, 0, 0, 0);
+    };
+    float acc[MT][NT][4] = {};
+    uint4 now[2 * MT], next[2 * MT];
+    fetch(c0 + wk, now);
+
+    const T* x = static_cast<const T*>(p.x) + r0 * p.ldx;
+    const int buffer = sp.stage * 16 * cols;  // 16-byte words of a stage
+    auto stage = [&](int first, uint4* to) {
+        const int runs = (min(first + sp.stage, c1) - first) * 16;
+        for (int i = threadIdx.x; i < runs * in_rows; i += kThreads) {
+            const int r = i / runs, run = i - r * runs;
+            int word, at;
+            place<MODE>(run & 15, &word, &at);
+            const size_t col = (size_t)first * kChunk + 8 * run;
+            stage_run(x + (size_t)r * p.ldx, col, col < (size_t)k, sp.vec, to + (((run >> 4) * 4 + word) * cols + r * P) * 4 + at, 4);
+        }
+    };
+    if (c0 < c1) stage(c0, s_x);
+    int b = 0;
+    for (int first = c0; first < c1; first += sp.stage, b ^= 1) {
+        __syncthreads();
+        const int last = min(first + sp.stage, c1);
+        if (last < c1) stage(last, s_x + (b ^ 1) * buffer);
+        for (int chunk = first + wk; chunk < last; chunk += sp.k_warps) {
+            fetch(chunk + sp.k_warps, next);
+            const uint4* xs = s_x + b * buffer + (size_t)(chunk - first) * 16 * cols + lane;
+            constexpr int kGroups = MODE == 0 ? 1 : 2 * MODE;  // of a chunk
+            const size_t group0 = MODE == 0 ? (size_t)chunk * kChunk / p.w.group : (size_t)chunk * kGroups;
+            float scale[2 * MT][kGroups];
+            uint32_t zero[2 * MT][kGroups];
+#pragma unroll
+            for (int m = 0; m < 2 * MT; ++m) {
+                by_group<MODE>(t, now[m]);
+#pragma unroll
+                for (int q = 0; q < kGroups; ++q) {
+                    const bool in = 8 * m < left && (MODE == 0 || group0 + q < p.w.groups);
+                    scale[m][q] = in ? load_f32(p.w.scales, p.w.scale_dtype, scale0 + m * 8 * p.w.groups + group0 + q) : 0.0f;
+                    zero[m][q] = kMagic | (!p.w.zeros ? 0x00080008u : in ? (uint32_t)p.w.zeros[scale0 + m * 8 * p.w.groups + group0 + q] * 0x00010001u : 0u);
+                }
+            }
+            float part[MT][NT][4] = {};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                constexpr int kWords = 4 / kGroups;  // of a group
+                const int q = i / kWords;
+                uint32_t a[MT][8];  // the word's registers of rows g and g + 8
+#pragma unroll
+                for (int m = 0; m < 2 * MT; ++m) {
+                    const uint32_t w = i == 0 ? now[m].x : i == 1 ? now[m].y : i == 2 ? now[m].z : now[m].w;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) a[m >> 1][2 * j + (m & 1)] = minus2<T>((w >> 4 * j & 0x000f000fu) | kMagic, zero[m][q]);
+                }
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    const uint4 v = j * 8 + g < cols ? xs[(i * cols + j * 8) * 4] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) {
+                        mma16816<T>(part[m][j], a[m][0], a[m][1], a[m][2], a[m][3], v.x, v.y);
+                        mma16816<T>(part[m][j], a[m][4], a[m][5], a[m][6], a[m][7], v.z, v.w);
+                    }
+                }
+                if ((i + 1) % kWords == 0) {  // a group's sums, or a chunk's of a longer group, meet their scale
+#pragma unroll
+                    for (int j = 0; j < NT; ++j)
+#pragma unroll
+                        for (int m = 0; m < MT; ++m)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                acc[m][j][e] = fmaf(part[m][j][e], scale[2 * m + (e >> 1)][q], acc[m][j][e]);
+                                part[m][j][e] = 0.0f;
+                            }
+                }
+            }
+#pragma unroll
+            for (int m = 0; m < 2 * MT; ++m) now[m] = next[m];
         }
     }
+    // the warps' sums side by side in shared memory, [k_warps][cta_rows][cols]
+    __syncthreads();
+    float* red = reinterpret_cast<float*>(s_x);
+    const int tile = cta_rows * cols;
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int row = (wm * MT + m) * 16 + (e >> 1) * 8 + g, col = j * 8 + 2 * t + (e & 1);
+                if (col < cols) red[wk * tile + row * cols + col] = acc[m][j][e];
+            }
+    __syncthreads();
+    namespace cg = cooperative_groups;
+    const cg::cluster_group cluster = cg::this_cluster();
+    const int ctas = gridDim.x;
+    if (ctas > 1) {
+        for (int i = threadIdx.x; i < tile; i += kThreads) {
+            float v = red[i];
+            for (int w = 1; w < sp.k_warps; ++w) v += red[w * tile + i];
+            red[i] = v;
+        }
+        cluster.sync();
+    }
+    if (blockIdx.x == 0) {
+        T* out = static_cast<T*>(p.out) + r0 * p.ldo;
+        for (int i = threadIdx.x; i < cta_rows * in_rows; i += kThreads) {
+            const int r = i / cta_rows, row = i - r * cta_rows;
+            const size_t n = n0 + row;
+            if (n >= p.w.n) continue;
+            float v = 0.0f;
+#pragma unroll
+            for (int piece = 0; piece < P; ++piece) {
+                const int at = row * cols + r * P + piece;
+                float u = red[at];
+                if (ctas > 1)
+                    for (int c = 1; c < ctas; ++c) u += cluster.map_shared_rank(red, c)[at];
+                else
+                    for (int w = 1; w < sp.k_warps; ++w) u += red[w * tile + at];
+                v = piece == 0 ? u : v + u;
+            }
+            T* o = out + (size_t)r * p.ldo + n;
+            *o = from_f32<T>(apply_epilogue(p.epilogue, v, p.alpha, p.epilogue == EPI_ADD_OUT ? to_f32(*o) : 0.0f));
+        }
+    }
+    if (ctas > 1) cluster.sync();  // no CTA leaves while its sums are read
 }
 
 __device__ __forceinline__ void store_scale(void* scales, int dtype, size_t i, float v) {
@@ -94,11 +362,55 @@ int32_t launch_w4_quantize(pssa_b200_ctx* ctx, const W4Params& w, const void* sr
     return after_launch(ctx, "w4_quantize_kernel");
 }
 
-int32_t launch_gemv_w4(pssa_b200_ctx* ctx, const GemvW4Params& p) {
-    const size_t blocks = (p.w.n * 32 + kThreads - 1) / kThreads;
-    if (blocks > 0x7fffffff) return fail(ctx, PSSA_B200_ERR_SHAPE, "B200 4-bit product: too many weight rows; refusing launch");
-    with_dtype(p.dtype, [&](auto t) { gemv_w4_kernel<decltype(t)><<<(unsigned)blocks, kThreads, 0, ctx->stream>>>(p); });
+namespace {
+template <typename T, int NT, int MT, int MODE>
+int32_t launch_tiles(pssa_b200_ctx* ctx, const GemvW4Params& p) {
+    constexpr int P = Mma<T>::pieces;
+    W4Split sp{};
+    sp.chunks = (int)((p.w.k + kChunk - 1) / kChunk);
+    sp.vec = (reinterpret_cast<uintptr_t>(p.x) & 15) == 0 && p.ldx * sizeof(T) % 16 == 0;
+    sp.slice = (int)std::min<size_t>(p.rows, NT * 8 / P);
+    sp.k_warps = NT >= 4 ? 2 : kWarps;
+    const int cta_rows = kWarps / sp.k_warps * MT * 16;
+    const size_t tiles = (p.w.n + cta_rows - 1) / cta_rows, slices = (p.rows + sp.slice - 1) / sp.slice;
+    if (tiles > 65535 || slices > 65535) return fail(ctx, PSSA_B200_ERR_SHAPE, "B200 4-bit product: too many rows; refusing launch");
+    int ctas = 1;
+    while (ctas < 8 && tiles * slices * ctas * 2 <= (size_t)ctx->sm_count * 2 && ctas * 2 * sp.k_warps <= sp.chunks) ctas *= 2;
+    sp.per_cta = (sp.chunks + ctas - 1) / ctas;
+    const size_t chunk_bytes = (size_t)16 * 16 * sp.slice * P, room = 48 * 1024;
+    sp.stage = (int)std::min<size_t>(sp.per_cta, std::max<size_t>(sp.k_warps, room / chunk_bytes / sp.k_warps * sp.k_warps));
+    const size_t smem = std::max(chunk_bytes * sp.stage * (sp.stage < sp.per_cta ? 2 : 1), (size_t)sp.k_warps * cta_rows * sp.slice * P * 4);
+    static PerDeviceOnce attr;
+    if (attr.need(ctx->device)) {
+        PSSA_CUDA(ctx, cudaFuncSetAttribute(gemv_w4_kernel<T, NT, MT, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
+        attr.done(ctx->device);
+    }
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(ctas, (unsigned)tiles, (unsigned)slices), cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = smem, cfg.stream = ctx->stream;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = ctas, at.val.clusterDim.y = 1, at.val.clusterDim.z = 1;
+    cfg.attrs = &at, cfg.numAttrs = 1;
+    PSSA_CUDA(ctx, cudaLaunchKernelEx(&cfg, gemv_w4_kernel<T, NT, MT, MODE>, p, sp));
     return after_launch(ctx, "gemv_w4_kernel");
+}
+}  // namespace
+
+int32_t launch_gemv_w4(pssa_b200_ctx* ctx, const GemvW4Params& p) {
+    return with_dtype(p.dtype, [&](auto t) -> int32_t {
+        using T = decltype(t);
+        auto by_group = [&](auto mode) {
+            constexpr int M = decltype(mode)::value;
+            const size_t cols = p.rows * Mma<T>::pieces;
+            if (cols <= 8) return launch_tiles<T, 1, 2, M>(ctx, p);
+            if (cols <= 16) return launch_tiles<T, 2, 2, M>(ctx, p);
+            if (cols <= 32) return launch_tiles<T, 4, 1, M>(ctx, p);
+            return launch_tiles<T, 8, 1, M>(ctx, p);
+        };
+        if (p.w.group == 32) return by_group(std::integral_constant<int, 2>());
+        if (p.w.group == 64) return by_group(std::integral_constant<int, 1>());
+        return by_group(std::integral_constant<int, 0>());
+    });
 }
 
 }  // namespace pssa
