@@ -1,129 +1,379 @@
 // Log probabilities of given tokens with rank, entropy and top alternatives, and their gradient (see pssa_b200_token_logprobs_dev).
-// One CTA per row, a pass over it for each thing that is asked.
-#include "element.cuh"
+//
+// Forward: one read of the row. Every thread keeps the running maximum, sum exp and sum exp * z of its vectors, counts the logits above the
+// target's, and remembers the lowest id of its maximum; the threads' and then the CTAs' numbers are joined in a fixed order. A few rows are split over the
+// CTAs of a cluster, which meet in distributed shared memory: one launch and no workspace whatever the shape.
+//
+// Alternatives come from the same pass. The n-th best of the threads' maxima (of pairs of neighbouring threads) bounds the n-th best logit from below,
+// and no logit above the bound lies outside the n pairs that reach it: only their shares, n / pairs of the row, are read again, and what is not
+// below the bound, hardly more than n logits, is sorted. Keys are (value, lower id first) and so never equal: ties change nothing. Where more pass
+// than there is room for (logits in an order made for it), the n are drawn one by one instead.
+#include <cooperative_groups.h>
+
+#include <type_traits>
+
 #include "kernels.hpp"
+#include "logit_row.cuh"
 
 namespace pssa {
 namespace {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr float kNan = __builtin_nanf("");
+namespace cg = cooperative_groups;
+using Key = unsigned long long;
 
-template <typename T, typename F>
-__device__ __forceinline__ T block_reduce(T v, T* scratch, F op) {
+constexpr int kRoom = 1024;  // candidates of a CTA
+
+struct RowPart {  // a CTA's numbers for its cluster
+    float top, ref, sum, ent;
+    unsigned above;
+};
+
+template <int THREADS>
+struct LogprobShared {
+    RowPart part;
+    float f[3][THREADS / 32];
+    unsigned u[THREADS / 32];
+    Key bound, wide[THREADS / 32];
+    int candidates;
+    Key pairs[THREADS / 2];
+    Key best[PSSA_B200_MAX_TOP];  // descending; 0 behind the last
+    Key found[kRoom];
+};
+
+template <int THREADS, typename V, typename F>
+__device__ __forceinline__ V block_reduce(V v, V* scratch, F op) {
 #pragma unroll
     for (int m = 16; m > 0; m >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, m));
-    __syncthreads();  // scratch may still be read from the previous call
+    __syncthreads();
     if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
     __syncthreads();
-    v = scratch[threadIdx.x & (kWarps - 1)];
+    v = scratch[threadIdx.x & (THREADS / 32 - 1)];
 #pragma unroll
-    for (int m = kWarps / 2; m > 0; m >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, m));
+    for (int m = THREADS / 64; m > 0; m >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, m));
     return v;
 }
 
-// ascending in (value, lower id first); -0 counts as +0
-__device__ __forceinline__ unsigned long long key_of(float x, int id) {
-    int b = __float_as_int(x + 0.0f);
-    b = b < 0 ? b ^ 0x7fffffff : b;
-    return (unsigned long long)(unsigned)(b ^ 0x80000000) << 32 | (0xffffffffu - (unsigned)id);
+// The part of a row that a CTA reads: vectors [v0, v1) of it, and the elements outside any vector: in front by the first CTA, behind by the last.
+template <typename T>
+struct Part {
+    const T* x;
+    const uint4* vec;
+    int head, v0, v1, tail0, n;
+    bool first, last;
+    __device__ Part(const T* row, int n_, int rank, int ctas) : x(row), n(n_), first(rank == 0), last(rank == ctas - 1) {
+        head = head_of(row, n);
+        const int vecs = (n - head) / kVec<T>, each = (vecs + ctas - 1) / ctas;
+        vec = reinterpret_cast<const uint4*>(row + head);
+        v0 = min(rank * each, vecs), v1 = min(v0 + each, vecs);
+        tail0 = head + vecs * kVec<T>;
+    }
+    // this thread's single element: its id, or -1
+    __device__ int single() const {
+        if (first && (int)threadIdx.x < head) return threadIdx.x;
+        const int i = tail0 + (int)threadIdx.x - kVec<T>;  // behind the heads' threads
+        return last && (int)threadIdx.x >= kVec<T> && i < n ? i : -1;
+    }
+};
+
+// The n best keys of the CTA's part into s.best. `own`: the thread's best key (0: it has none).
+template <typename T, int THREADS>
+__device__ void best_of_part(const Part<T>& part, Key own, int n, LogprobShared<THREADS>& s) {
+    constexpr int kPairs = THREADS / 2;
+    const int tid = threadIdx.x, single = part.single();
+    // the n-th best of the pairs' maxima
+    const Key mate = __shfl_xor_sync(0xffffffffu, own, 1);
+    if ((tid & 1) == 0) s.pairs[tid >> 1] = own > mate ? own : mate;
+    if (tid == 0) s.bound = 0, s.candidates = 0;
+    if (tid < PSSA_B200_MAX_TOP) s.best[tid] = 0;
+    __syncthreads();
+    if (tid < kPairs) {
+        const Key k = s.pairs[tid];
+        int better = 0;
+        for (int i = 0; i < kPairs; ++i) better += s.pairs[i] > k;
+        if (k != 0 && better == n - 1) s.bound = k;  // stays 0 where fewer pairs have a logit: then all are candidates
+    }
+    __syncthreads();
+    const Key bound = s.bound;
+    auto offer = [&](float x, int id) {
+        const Key k = key_of(x, id);
+        if (k >= bound) {
+            const int at = atomicAdd(&s.candidates, 1);
+            if (at < kRoom) s.found[at] = k;
+        }
+    };
+    if (single >= 0) offer(to_f32(part.x[single]), single);
+    // the shares of the pairs that reach the bound, dealt out anew: item (pair, vector of it)
+    const int steps = (part.v1 - part.v0 + THREADS - 1) / THREADS;
+    const float floor = bound == 0 ? -INFINITY : key_value(bound);
+    __shared__ short s_list[kPairs];
+    __shared__ int s_pairs;
+    if (tid == 0) s_pairs = 0;
+    __syncthreads();
+    if (tid < kPairs && s.pairs[tid] != 0 && s.pairs[tid] >= bound) s_list[atomicAdd(&s_pairs, 1)] = (short)tid;
+    __syncthreads();
+    const int items = s_pairs * steps * 2;
+    for (int i = tid; i < items; i += THREADS) {
+        const int step = (i >> 1) % steps, p = s_list[(i >> 1) / steps], v = part.v0 + step * THREADS + 2 * p + (i & 1);
+        if (v >= part.v1) continue;
+        float x[kVec<T>];
+        unpack<T>(part.vec[v], x);
+#pragma unroll
+        for (int e = 0; e < kVec<T>; ++e)
+            if (x[e] >= floor) offer(x[e], part.head + v * kVec<T> + e);
+    }
+    __syncthreads();
+    const int c = s.candidates;
+    if (c <= kRoom) {
+        for (int i = tid; i < c; i += THREADS) {
+            const Key k = s.found[i];
+            int better = 0;
+            for (int j = 0; j < c; ++j) better += s.found[j] > k;
+            if (better < n) s.best[better] = k;
+        }
+    } else {  // one by one; a thread looks its share over again when it has lost its best
+        for (int r = 0; r < n; ++r) {
+            const Key best = block_reduce<THREADS>(own, s.wide, [](Key a, Key b) { return a > b ? a : b; });
+            if (tid == 0) s.best[r] = best;
+            if (own == best && own != 0) {
+                own = 0;
+                auto look = [&](float x, int id) {
+                    const Key k = key_of(x, id);
+                    if (k < best && k > own) own = k;
+                };
+                for (int v = part.v0 + tid; v < part.v1; v += THREADS) {
+                    float x[kVec<T>];
+                    unpack<T>(part.vec[v], x);
+#pragma unroll
+                    for (int e = 0; e < kVec<T>; ++e) look(x[e], part.head + v * kVec<T> + e);
+                }
+                if (single >= 0) look(to_f32(part.x[single]), single);
+            }
+        }
+    }
+    __syncthreads();
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) token_logprobs_kernel(LogprobParams p) {
-    __shared__ float s_f[kWarps];
-    __shared__ unsigned s_u[kWarps];
-    __shared__ unsigned long long s_k[kWarps];
-    const size_t row = blockIdx.x;
+template <typename T, int THREADS, bool TOP>
+__global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LogprobParams p, int ctas) {
+    __shared__ LogprobShared<THREADS> s;
+    constexpr int kWarps = THREADS / 32, N = kVec<T>, kAhead = 4;
+    const size_t row = blockIdx.x / (unsigned)ctas;
+    const int rank = blockIdx.x % (unsigned)ctas, tid = threadIdx.x, warp = tid >> 5;
     const T* x = static_cast<const T*>(p.logits) + row * p.ld;
-    const int v = p.vocab, tid = threadIdx.x;
-    const float inv_t = 1.0f / p.temperature;
-    auto sum = [](auto a, auto b) { return a + b; };
-    float m = -INFINITY;
-    unsigned bad = 0;
-    for (int i = tid; i < v; i += kThreads) {
-        const float a = to_f32(x[i]);
-        bad |= !(a < INFINITY);
-        m = fmaxf(m, a);
-    }
-    bad = block_reduce(bad, s_u, [](unsigned a, unsigned b) { return a | b; });
-    m = block_reduce(m, s_f, [](float a, float b) { return fmaxf(a, b); });
+    const int v = p.vocab;
+    const Part<T> part(x, v, rank, ctas);
+    const float inv_t = 1.0f / p.temperature, c = kLog2e / p.temperature;
     const uint32_t t = p.targets ? p.targets[row] : PSSA_B200_NO_TOKEN;
     const bool has = t < (uint32_t)v, none = t == PSSA_B200_NO_TOKEN;
-    if (!has && !none && tid == 0) atomicExch(p.status, PSSA_B200_ERR_TOKEN);
-    const bool empty = m == -INFINITY;
-    const float xt = has ? to_f32(x[t]) : 0.0f;
-    float s = 0.0f, e = 0.0f;
+    const float xt = has ? to_f32(x[t]) : INFINITY;
+
+    SoftmaxSums<true> sums;
     unsigned above = 0;
-    for (int i = tid; i < v; i += kThreads) {
-        const float a = to_f32(x[i]), z = empty ? -INFINITY : (a - m) * inv_t, w = expf(z);
-        s += w;
-        if (w > 0.0f) e += w * z;
-        above += has && a > xt;
+    auto take = [&](uint4 raw, int at) {
+        float f[N];
+        unpack<T>(raw, f);
+        sums.add(f, part.head + at * N, c);
+        float m = f[0];
+#pragma unroll
+        for (int i = 1; i < N; ++i) m = fmaxf(m, f[i]);
+        if (m > xt) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) above += f[i] > xt;
+        }
+    };
+    int at = part.v0 + tid;
+    if (TOP) {  // until something is above -inf the lowest id of the share is its best
+        const int i = part.single();
+        sums.id = i >= 0 && i < part.head ? i : at < part.v1 ? part.head + at * N : i;
     }
-    s = block_reduce(s, s_f, sum);
-    e = block_reduce(e, s_f, sum);
-    above = block_reduce(above, s_u, sum);
-    const float ls = empty ? 0.0f : logf(s);
-    auto logp = [&](float a) { return bad ? kNan : empty ? -INFINITY : (a - m) * inv_t - ls; };
+    for (; at + (kAhead - 1) * THREADS < part.v1; at += kAhead * THREADS) {
+        uint4 raw[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) raw[i] = part.vec[at + i * THREADS];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) take(raw[i], at + i * THREADS);
+    }
+    for (; at < part.v1; at += THREADS) take(part.vec[at], at);
+    if (const int i = part.single(); i >= 0) {
+        const float f = to_f32(x[i]);
+        // a head's ids are below, a tail's above all others of the thread: the lowest id of the best stays right
+        if (f == sums.top && i < sums.id) sums.id = i;
+        sums.add1(f, i, c);
+        above += f > xt;
+    }
+    // the CTA's numbers
+    const float ref = block_reduce<THREADS>(sums.ref, s.f[0], [](float a, float b) { return fmaxf(a, b); });
+    const float top = block_reduce<THREADS>(sums.top, s.f[0], [](float a, float b) { return fmaxf(a, b); });
+    float sum = sums.total(), ent = sums.entropy_total();
+    rebase(sums.ref, ref, c, sum, ent);
+#pragma unroll
+    for (int m = 16; m > 0; m >>= 1) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, m);
+        ent += __shfl_xor_sync(0xffffffffu, ent, m);
+        above += __shfl_xor_sync(0xffffffffu, above, m);
+    }
+    if ((tid & 31) == 0) s.f[1][warp] = sum, s.f[2][warp] = ent, s.u[warp] = above;
+    __syncthreads();
     if (tid == 0) {
-        if (p.logprob) p.logprob[row] = none ? 0.0f : has ? logp(xt) : kNan;
-        if (p.rank) p.rank[row] = bad || !has ? 0 : above + 1;
-        if (p.entropy) p.entropy[row] = bad ? kNan : empty ? 0.0f : ls - e / s;
-        if (p.stats) p.stats[2 * row] = bad ? kNan : m, p.stats[2 * row + 1] = bad ? kNan : ls;
+        sum = ent = 0.0f, above = 0;
+        for (int i = 0; i < kWarps; ++i) sum += s.f[1][i], ent += s.f[2][i], above += s.u[i];
+        s.part = RowPart{top, ref, sum, ent, above};
     }
-    unsigned long long last = ~0ull;
-    for (int n = 0; n < p.top_n; ++n) {
-        unsigned long long best = 0;
-        for (int i = tid; i < v; i += kThreads) {
-            const unsigned long long k = key_of(to_f32(x[i]), i);
-            if (k < last && k > best) best = k;
+    if (TOP) best_of_part<T, THREADS>(part, sums.id >= 0 ? key_of(sums.top, sums.id) : 0, p.top_n, s);
+    // the cluster's
+    const cg::cluster_group cluster = cg::this_cluster();
+    if (ctas > 1)
+        cluster.sync();
+    else
+        __syncthreads();
+    if (rank == 0) {
+        RowPart all = s.part;
+        for (int i = 1; i < ctas; ++i) {
+            RowPart o = *cluster.map_shared_rank(&s.part, i);
+            const float to = fmaxf(all.ref, o.ref);
+            rebase(all.ref, to, c, all.sum, all.ent);
+            rebase(o.ref, to, c, o.sum, o.ent);
+            all.ref = to, all.top = fmaxf(all.top, o.top), all.sum += o.sum, all.ent += o.ent, all.above += o.above;
         }
-        best = block_reduce(best, s_k, [](unsigned long long a, unsigned long long b) { return a > b ? a : b; });
-        last = best;
+        const bool bad = all.sum != all.sum || all.top == INFINITY, empty = all.top == -INFINITY;
+        const float ls = empty ? 0.0f : logf(all.sum);
+        auto logp = [&](float a) { return bad ? kNan : empty ? -INFINITY : (a - all.top) * inv_t - ls; };
         if (tid == 0) {
-            const unsigned id = 0xffffffffu - (unsigned)best;
-            const bool there = n < v && !bad;
-            p.top_ids[row * p.top_n + n] = there ? id : PSSA_B200_NO_TOKEN;
-            p.top_logprobs[row * p.top_n + n] = bad ? kNan : there ? logp(to_f32(x[id])) : -INFINITY;
+            if (!has && !none) atomicExch(p.status, PSSA_B200_ERR_TOKEN);
+            if (p.logprob) p.logprob[row] = none ? 0.0f : has ? logp(xt) : kNan;
+            if (p.rank) p.rank[row] = bad || !has ? 0 : all.above + 1;
+            if (p.entropy) p.entropy[row] = bad ? kNan : empty ? 0.0f : ls - kLn2 * (all.ent / all.sum);
+            if (p.stats) p.stats[2 * row] = bad ? kNan : all.top, p.stats[2 * row + 1] = bad ? kNan : ls;
         }
+        if (TOP) {
+            const int n = p.top_n;
+            auto put = [&](int r, Key k) {
+                p.top_ids[row * n + r] = k && !bad ? key_id(k) : PSSA_B200_NO_TOKEN;
+                p.top_logprobs[row * n + r] = bad ? kNan : k ? logp(key_value(k)) : -INFINITY;
+            };
+            if (ctas == 1) {
+                if (tid < n) put(tid, s.best[tid]);
+            } else {  // a key's place is the number of better ones: its own list is in order, the others are searched
+                for (int i = tid; i < n * ctas; i += THREADS) {
+                    const int list = i / n, at_ = i - list * n;
+                    const Key k = cluster.map_shared_rank(s.best, list)[at_];
+                    if (k == 0) continue;
+                    int place = at_;
+                    for (int l = 0; l < ctas; ++l) {
+                        if (l == list) continue;
+                        const Key* o = cluster.map_shared_rank(s.best, l);
+                        int lo = 0, hi = n;  // the first that is not better
+                        while (lo < hi) {
+                            const int mid = (lo + hi) >> 1;
+                            if (o[mid] > k)
+                                lo = mid + 1;
+                            else
+                                hi = mid;
+                        }
+                        place += lo;
+                    }
+                    if (place < n) put(place, k);
+                }
+                for (int r = v + tid; r < n; r += THREADS) put(r, 0);  // fewer ids than places
+            }
+        }
+    }
+    if (ctas > 1) cluster.sync();  // no CTA leaves while its numbers are read
+}
+
+// d = p (A + B lp) + (at the target) g, lp = log2 p: one read, one write. A CTA takes `span` vectors of one row; rows that start at different
+// distances from a 16-byte boundary in the two arrays go element by element.
+constexpr int kGradThreads = 256, kGradAhead = 4;
+
+template <typename T>
+__global__ void __launch_bounds__(kGradThreads) token_logprobs_grad_kernel(LogprobGradParams p, unsigned spans) {
+    constexpr int N = kVec<T>;
+    const size_t row = blockIdx.x / spans;
+    const int span = blockIdx.x % spans, tid = threadIdx.x, v = p.vocab;
+    const T* x = static_cast<const T*>(p.logits) + row * p.ld;
+    T* out = static_cast<T*>(p.grad) + row * p.ld_grad;
+    const bool together = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
+    const int head = together ? head_of(x, v) : v, vecs = (v - head) / N, tail0 = head + vecs * N;
+    const uint4* xv = reinterpret_cast<const uint4*>(x + head);
+    uint4* ov = reinterpret_cast<uint4*>(out + head);
+    const int v0 = span * kGradThreads * kGradAhead + tid;
+    uint4 raw[kGradAhead];
+#pragma unroll
+    for (int i = 0; i < kGradAhead; ++i)
+        if (v0 + i * kGradThreads < vecs) raw[i] = xv[v0 + i * kGradThreads];
+
+    const float inv_t = 1.0f / p.temperature, c = kLog2e / p.temperature;
+    const uint32_t t = p.targets ? p.targets[row] : PSSA_B200_NO_TOKEN;
+    const bool has = t < (uint32_t)v;
+    const float w_lp = has && p.grad_logprob ? p.grad_logprob[row] : 0.0f, w_h = p.grad_entropy ? p.grad_entropy[row] : 0.0f;
+    const float m = p.stats[2 * row], l2 = p.stats[2 * row + 1] * kLog2e, h = p.grad_entropy ? p.entropy[row] : 0.0f;
+    const bool zero = (w_lp == 0.0f && w_h == 0.0f) || m == -INFINITY;
+    const float g = w_lp * inv_t, a = -(g + w_h * inv_t * h), b = -w_h * inv_t * kLn2;
+    if (span == 0 && tid == 0 && !has && t != PSSA_B200_NO_TOKEN) atomicExch(p.status, PSSA_B200_ERR_TOKEN);
+    auto one = [&](float f) {
+        const float lp = fmaf(f - m, c, -l2), pr = ex2(lp);
+        // the lowest power that is not 0 is -149: below it the bracket only has to be finite. A NaN stays one through ex2.
+        return pr * fmaf(b, fmaxf(lp, -200.0f), a);
+    };
+#pragma unroll
+    for (int i = 0; i < kGradAhead; ++i) {
+        const int at = v0 + i * kGradThreads;
+        if (at >= vecs) break;
+        float f[N];
+        unpack<T>(raw[i], f);
+#pragma unroll
+        for (int e = 0; e < N; ++e) f[e] = zero ? 0.0f : one(f[e]);
+        const unsigned off = t - (unsigned)(head + at * N);
+        if (off < (unsigned)N && !zero) {
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                if (off == (unsigned)e) f[e] += g;
+        }
+        ov[at] = pack<T>(f);
+    }
+    auto single = [&](int i) { out[i] = from_f32<T>(zero ? 0.0f : one(to_f32(x[i])) + ((unsigned)i == t ? g : 0.0f)); };
+    if (!together) {
+        for (int i = span * kGradThreads * kGradAhead * N + tid; i < min((span + 1) * kGradThreads * kGradAhead * N, v); i += kGradThreads) single(i);
+    } else if (span == 0) {
+        if (tid < head) single(tid);
+        if (tail0 + tid < v) single(tail0 + tid);
     }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) token_logprobs_grad_kernel(LogprobGradParams p) {
-    const size_t row = blockIdx.x;
-    const T* x = static_cast<const T*>(p.logits) + row * p.ld;
-    T* g = static_cast<T*>(p.grad) + row * p.ld_grad;
-    const int v = p.vocab, tid = threadIdx.x;
-    const float inv_t = 1.0f / p.temperature;
-    const uint32_t t = p.targets ? p.targets[row] : PSSA_B200_NO_TOKEN;
-    const bool has = t < (uint32_t)v;
-    if (!has && t != PSSA_B200_NO_TOKEN && tid == 0) atomicExch(p.status, PSSA_B200_ERR_TOKEN);
-    const float g_lp = has && p.grad_logprob ? p.grad_logprob[row] * inv_t : 0.0f;
-    const float g_h = p.grad_entropy ? p.grad_entropy[row] * inv_t : 0.0f;
-    const float m = p.stats[2 * row], ls = p.stats[2 * row + 1], h = p.grad_entropy ? p.entropy[row] : 0.0f;
-    const bool zero = (g_lp == 0.0f && g_h == 0.0f) || m == -INFINITY;
-    for (int i = tid; i < v; i += kThreads) {
-        float d = 0.0f;
-        if (!zero) {
-            const float lp = (to_f32(x[i]) - m) * inv_t - ls, pr = expf(lp);
-            d = g_lp * ((i == (int)t ? 1.0f : 0.0f) - pr);
-            if (pr != 0.0f) d -= g_h * (pr * (lp + h));
-        }
-        g[i] = from_f32<T>(d);
-    }
+template <typename T, int THREADS, bool TOP>
+cudaError_t launch_rows(pssa_b200_ctx* ctx, const LogprobParams& p, int ctas) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(p.rows * ctas)), cfg.blockDim = dim3(THREADS), cfg.stream = ctx->stream;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = ctas, at.val.clusterDim.y = 1, at.val.clusterDim.z = 1;
+    cfg.attrs = &at, cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, THREADS, TOP>, p, ctas);
 }
 
 }  // namespace
 
 int32_t launch_token_logprobs(pssa_b200_ctx* ctx, const LogprobParams& p) {
-    with_dtype(p.dtype, [&](auto t) { token_logprobs_kernel<decltype(t)><<<(unsigned)p.rows, kThreads, 0, ctx->stream>>>(p); });
+    const size_t vecs = (size_t)p.vocab * dtype_size(p.dtype) / 16;
+    int ctas = 1;  // of a row: until the GPU has two of them to an SM, or a thread would have no vector left
+    while (ctas < 8 && p.rows * ctas < (size_t)ctx->sm_count * 2 && vecs / (ctas * 2) >= 256) ctas *= 2;
+    const bool few = p.rows * ctas <= (size_t)ctx->sm_count && vecs / ctas >= 2048;  // more threads, where few CTAs have long parts
+    if (p.rows * ctas > 0x7fffffffull) return fail(ctx, PSSA_B200_ERR_SHAPE, "B200 log probabilities: too many rows; refusing launch");
+    const cudaError_t e = with_dtype(p.dtype, [&](auto t) {
+        using T = decltype(t);
+        if (few) return p.top_n ? launch_rows<T, 1024, true>(ctx, p, ctas) : launch_rows<T, 1024, false>(ctx, p, ctas);
+        return p.top_n ? launch_rows<T, 256, true>(ctx, p, ctas) : launch_rows<T, 256, false>(ctx, p, ctas);
+    });
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "token_logprobs_kernel");
     return after_launch(ctx, "token_logprobs_kernel");
 }
 
 int32_t launch_token_logprobs_grad(pssa_b200_ctx* ctx, const LogprobGradParams& p) {
-    with_dtype(p.dtype, [&](auto t) { token_logprobs_grad_kernel<decltype(t)><<<(unsigned)p.rows, kThreads, 0, ctx->stream>>>(p); });
+    const size_t per = (size_t)kGradThreads * kGradAhead * 16 / dtype_size(p.dtype), spans = (p.vocab + per - 1) / per;
+    if (p.rows * spans > 0x7fffffffull) return fail(ctx, PSSA_B200_ERR_SHAPE, "B200 log probabilities' gradient: too many rows; refusing launch");
+    with_dtype(p.dtype, [&](auto t) {
+        token_logprobs_grad_kernel<decltype(t)><<<(unsigned)(p.rows * spans), kGradThreads, 0, ctx->stream>>>(p, (unsigned)spans);
+    });
     return after_launch(ctx, "token_logprobs_grad_kernel");
 }
 
