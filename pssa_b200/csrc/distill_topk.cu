@@ -1,14 +1,28 @@
 // Distillation from a teacher's best ids: divergence, a target's cross entropy and the gradient in one call (see
-// pssa_b200_distill_topk_dev). One CTA per row; the listed ids are marked in a bitmap, so that the mass of the ids that are not
-// listed is summed by itself and never the difference of two numbers near 1.
-#include "element.cuh"
+// pssa_b200_distill_topk_dev).
+//
+// A row of logits is read once and its gradient written once: a cluster of CTAs holds the row in shared memory between the pass that sums
+// and the pass that writes. The listed ids' logits are fetched on the side and then masked in shared memory, so that the pass sums the ids that are
+// not listed by themselves: the mass of the rest is never the difference of two numbers near 1, and a student that is sure of the listed ids gets its
+// gradient relative to the rest's own maximum. The listed ids, at most 256, are added by the thread that holds the entry, and their gradient is written over
+// the zeros that the pass left there. Every CTA of a cluster does the entries' arithmetic for itself, in the same order and so to the same bits.
+//
+// Vocabularies whose row does not fit a cluster's shared memory take the second kernel: one CTA per row, a pass over global memory for each
+// thing, the listed ids marked in a bitmap.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+#include <type_traits>
+
 #include "kernels.hpp"
+#include "logit_row.cuh"
+#include "tcgen05.cuh"
 
 namespace pssa {
 namespace {
 
+namespace cg = cooperative_groups;
 constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr float kNan = __builtin_nanf("");
 
 template <typename T, typename F>
 __device__ __forceinline__ T block_reduce(T v, T* scratch, F op) {
@@ -24,7 +38,7 @@ __device__ __forceinline__ T block_reduce(T v, T* scratch, F op) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) distill_topk_kernel(DistillParams p) {
+__global__ void __launch_bounds__(kThreads) distill_topk_long_kernel(DistillParams p) {
     extern __shared__ unsigned s_bits[];
     __shared__ float s_f[kWarps], s_x[PSSA_B200_MAX_TEACHER], s_t[PSSA_B200_MAX_TEACHER];
     __shared__ double s_d[kWarps];
@@ -127,20 +141,234 @@ __global__ void __launch_bounds__(kThreads) distill_topk_kernel(DistillParams p)
     }
 }
 
+struct RestSums {  // of a CTA's unlisted ids: sums at the temperature, and at 1
+    float top, ref, sum, sum1;
+};
+
+// A CTA holds elements [rank * each, + each) of a row, at the distance from a 16-byte boundary that they have in global memory.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) distill_topk_kernel(DistillParams p, int ctas, int each) {
+    extern __shared__ __align__(128) unsigned char s_raw[];
+    __shared__ float s_f[kWarps], s_t[PSSA_B200_MAX_TEACHER];
+    __shared__ double s_d[kWarps];
+    __shared__ unsigned s_id[PSSA_B200_MAX_TEACHER];
+    __shared__ RestSums s_part;
+    __shared__ __align__(8) uint64_t s_bar;
+    constexpr int N = kVec<T>;
+    const size_t row = blockIdx.x / (unsigned)ctas;
+    const int rank = blockIdx.x % (unsigned)ctas, tid = threadIdx.x, v = p.vocab;
+    const T* x = static_cast<const T*>(p.logits) + row * p.ld;
+    auto sum = [](auto a, auto b) { return a + b; };
+    auto most = [](float a, float b) { return fmaxf(a, b); };
+
+    // the part, on its way to shared memory: whole 16-byte pieces by one bulk copy, what lies around them by single loads
+    const int e0 = min(rank * each, v), e1 = min(e0 + each, v), n = e1 - e0;
+    const T* from = x + e0;
+    const int off = (int)(reinterpret_cast<uintptr_t>(from) & 15) / (int)sizeof(T), head = off ? min(N - off, n) : 0;
+    const int vecs = (n - head) / N, tail0 = head + vecs * N;
+    T* held = reinterpret_cast<T*>(s_raw) + off;
+    uint4* held_vec = reinterpret_cast<uint4*>(held + head);
+    if (tid == 0) {
+        tc::mbar_init(&s_bar, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        if (vecs) {
+            tc::mbar_expect_tx(&s_bar, vecs * 16);
+            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(tc::smem_u32(held_vec)),
+                         "l"(from + head), "r"(vecs * 16), "r"(tc::smem_u32(&s_bar))
+                         : "memory");
+        }
+    }
+    if (tid < head) held[tid] = from[tid];
+    if (tail0 + tid < n) held[tail0 + tid] = from[tail0 + tid];
+
+    // the teacher's entries, one to a thread
+    const float inv_t = 1.0f / p.temperature, c = kLog2e / p.temperature;
+    const uint32_t id = tid < p.k ? p.teacher_ids[row * p.k + tid] : PSSA_B200_NO_TOKEN;
+    const uint32_t tgt = p.targets ? p.targets[row] : PSSA_B200_NO_TOKEN;
+    const bool entry = id < (uint32_t)v, has = tgt < (uint32_t)v, none = tgt == PSSA_B200_NO_TOKEN;
+    const float w_kl = p.grad_kl ? p.grad_kl[row] : 0.0f, w_ce = p.grad_ce && has ? p.grad_ce[row] : 0.0f;
+    const float xe = entry ? to_f32(x[id]) : -INFINITY, xt = has ? to_f32(x[tgt]) : -INFINITY;
+    const float q = entry ? p.teacher[row * p.k + tid] * (1.0f / p.teacher_temperature) : -INFINITY;
+    if (rank == 0 && ((!entry && id != PSSA_B200_NO_TOKEN) || (tid == 0 && !has && !none))) atomicExch(p.status, PSSA_B200_ERR_TOKEN);
+    float t, log_t = q, r = 0.0f;
+    if (p.rest) {
+        t = entry ? expf(q) : 0.0f;
+        r = fmaxf((float)(1.0 - block_reduce(entry ? exp((double)q) : 0.0, s_d, sum)), 0.0f);
+        if (!__syncthreads_or(entry)) r = 0.0f;  // no entry: nothing to learn
+    } else {
+        const float mt = block_reduce(entry && q != q ? INFINITY : q, s_f, most);  // a NaN goes through the sum
+        const float e = entry && mt > -INFINITY ? expf(q - mt) : 0.0f;
+        const float st = block_reduce(e, s_f, sum);
+        t = st != 0.0f ? e / st : 0.0f;
+        log_t = q - mt - logf(st);
+    }
+    s_id[tid] = entry ? id : PSSA_B200_NO_TOKEN;
+    s_t[tid] = t;
+    __syncthreads();  // also: the barrier is ready for every thread
+    bool first = entry;  // of the entries with its id
+    float t_at = 0.0f;
+    if (entry)
+        for (int j = 0; j < p.k; ++j)
+            if (s_id[j] == id) {
+                first = first && j >= tid;
+                t_at += s_t[j];
+            }
+    if (vecs && !tc::mbar_wait(&s_bar, 0)) {
+        atomicExch(p.status, PSSA_B200_ERR_TIMEOUT);
+        tc::mbar_wait(&s_bar, 0);  // no CTA leaves with its copy on the way, if a wait can help it
+    }
+    const bool mine = entry && id >= (uint32_t)e0 && id < (uint32_t)e1;
+    if (mine) held[id - e0] = from_f32<T>(-INFINITY);
+    __syncthreads();
+
+    // the sums of the ids that are not listed; at temperature 1 they serve the cross entropy too
+    const bool two = p.targets && p.temperature != 1.0f;
+    SoftmaxSums<false> rest, rest1;
+    for (int i = tid; i < vecs; i += kThreads) {
+        float f[N];
+        unpack<T>(held_vec[i], f);
+        rest.add(f, 0, c);
+        if (two) rest1.add(f, 0, kLog2e);
+    }
+    auto single = [&](int i) {
+        const float f = to_f32(held[i]);
+        rest.add1(f, 0, c);
+        if (two) rest1.add1(f, 0, kLog2e);
+    };
+    if (tid < head) single(tid);
+    if (tail0 + tid < n) single(tail0 + tid);
+    const float p_ref = block_reduce(rest.ref, s_f, most), p_top = block_reduce(rest.top, s_f, most);
+    float part = rest.total(), part1 = rest1.total(), unused = 0.0f;
+    rebase(rest.ref, p_ref, c, part, unused);
+    rebase(rest1.ref, p_ref, kLog2e, part1, unused);
+    part = block_reduce(part, s_f, sum);
+    if (two) part1 = block_reduce(part1, s_f, sum);
+    if (tid == 0) s_part = RestSums{p_top, p_ref, part, two ? part1 : part};
+    const cg::cluster_group cluster = cg::this_cluster();
+    if (ctas > 1)
+        cluster.sync();
+    else
+        __syncthreads();
+    RestSums all = s_part;
+    if (ctas > 1) {
+        all = *cluster.map_shared_rank(&s_part, 0);
+        for (int i = 1; i < ctas; ++i) {
+            RestSums o = *cluster.map_shared_rank(&s_part, i);
+            const float to = fmaxf(all.ref, o.ref);
+            rebase(all.ref, to, c, all.sum, unused);
+            rebase(o.ref, to, c, o.sum, unused);
+            rebase(all.ref, to, kLog2e, all.sum1, unused);
+            rebase(o.ref, to, kLog2e, o.sum1, unused);
+            all.ref = to, all.top = fmaxf(all.top, o.top), all.sum += o.sum, all.sum1 += o.sum1;
+        }
+    }
+    // with the listed ids: everything relative to the row's maximum m, the rest's sum to its own
+    const float xe_max = block_reduce(xe, s_f, most), m = fmaxf(all.top, xe_max);
+    const bool bad = __syncthreads_or(xe != xe) || all.sum != all.sum || m == INFINITY, empty = m == -INFINITY;
+    const float z = empty ? -INFINITY : (xe - m) * inv_t;
+    const float to_m = empty ? 0.0f : fmaxf(all.ref - m, -FLT_MAX);
+    const float s = all.sum * ex2(to_m * c) + block_reduce(first ? expf(z) : 0.0f, s_f, sum);
+    const float ls = logf(s);
+    const float log_rest = to_m * inv_t + logf(all.sum) - ls, p_rest = expf(log_rest);
+    float s1 = s;
+    if (two) s1 = all.sum1 * ex2(to_m * kLog2e) + block_reduce(first ? expf(empty ? -INFINITY : xe - m) : 0.0f, s_f, sum);
+    const float mass = block_reduce(t, s_f, sum) + r;
+    if (rank == 0) {
+        const float term = t > 0.0f || t != t ? t * (log_t - (empty ? -INFINITY : z - ls)) : 0.0f;
+        float kl = block_reduce(term, s_f, sum);
+        if (r > 0.0f) kl += r * (logf(r) - (empty || all.sum == 0.0f ? -INFINITY : log_rest));
+        if (tid == 0) {
+            if (p.kl) p.kl[row] = bad ? kNan : kl;
+            if (p.ce) p.ce[row] = none ? 0.0f : bad || !has ? kNan : empty ? INFINITY : logf(s1) - (xt - m);
+        }
+    }
+    if (ctas > 1) cluster.sync();  // the other CTAs' sums have been read, and all logits that lie where the gradient goes
+    if (!p.grad) return;
+    const bool zero = (w_kl == 0.0f && w_ce == 0.0f) || (empty && !bad);
+    const float g = w_kl * inv_t;
+    // an unlisted id: its share of the rest, times a, and its probability at temperature 1
+    const float a = all.sum > 0.0f ? g * (p.rest ? mass * p_rest - r : mass * p_rest) / all.sum : 0.0f;
+    const float a1 = w_ce * ex2(to_m * kLog2e) / s1;
+    const float both = two ? a : a + a1;
+    T* out = static_cast<T*>(p.grad) + row * p.ld_grad + e0;
+    const bool ce2 = two && w_ce != 0.0f;
+    auto grad = [&](float f) {
+        const float d = f - all.ref;
+        float y = both * ex2(d * c);
+        if (ce2) y = fmaf(a1, ex2(d * kLog2e), y);
+        return zero ? 0.0f : bad ? kNan : y;
+    };
+    const bool together = ((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(from)) & 15) == 0;
+    if (together) {
+        uint4* out_vec = reinterpret_cast<uint4*>(out + head);
+        for (int i = tid; i < vecs; i += kThreads) {
+            float f[N];
+            unpack<T>(held_vec[i], f);
+#pragma unroll
+            for (int e = 0; e < N; ++e) f[e] = grad(f[e]);
+            out_vec[i] = pack<T>(f);
+        }
+        if (tid < head) out[tid] = from_f32<T>(grad(to_f32(held[tid])));
+        if (tail0 + tid < n) out[tail0 + tid] = from_f32<T>(grad(to_f32(held[tail0 + tid])));
+    } else {
+        for (int i = tid; i < n; i += kThreads) out[i] = from_f32<T>(grad(to_f32(held[i])));
+    }
+    if (bad || zero) return;
+    __syncthreads();  // the listed ids and the target go over what has been written
+    bool at_target = false;
+    if (mine && first) {
+        float d = g * (mass * (expf(z) / s) - t_at);
+        if (w_ce != 0.0f) {
+            at_target = id == tgt;
+            d += w_ce * (expf(xe - m) / s1 - (at_target ? 1.0f : 0.0f));
+        }
+        out[id - e0] = from_f32<T>(d);
+    }
+    const bool listed = __syncthreads_or(entry && id == tgt);
+    if (tid == 0 && w_ce != 0.0f && !listed && tgt >= (uint32_t)e0 && tgt < (uint32_t)e1) out[tgt - e0] = from_f32<T>(grad(xt) - w_ce);
+}
+
+template <typename T>
+int32_t launch_parts(pssa_b200_ctx* ctx, const DistillParams& p, int ctas) {
+    // parts end on multiples of 16 bytes of the row, not of memory: rows may start anywhere
+    const size_t each = ((p.vocab + ctas - 1) / ctas + kVec<T> - 1) / kVec<T> * kVec<T>, smem = (each + kVec<T>) * sizeof(T);
+    static PerDeviceOnce attr;
+    if (attr.need(ctx->device)) {
+        PSSA_CUDA(ctx, cudaFuncSetAttribute(distill_topk_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
+        attr.done(ctx->device);
+    }
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(p.rows * ctas)), cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = smem, cfg.stream = ctx->stream;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = ctas, at.val.clusterDim.y = 1, at.val.clusterDim.z = 1;
+    cfg.attrs = &at, cfg.numAttrs = 1;
+    PSSA_CUDA(ctx, cudaLaunchKernelEx(&cfg, distill_topk_kernel<T>, p, ctas, (int)each));
+    return after_launch(ctx, "distill_topk_kernel");
+}
+
 }  // namespace
 
 int32_t launch_distill_topk(pssa_b200_ctx* ctx, const DistillParams& p) {
+    const size_t bytes = (size_t)p.vocab * dtype_size(p.dtype);
+    if (bytes <= 8 * 192 * 1024) {
+        // parts of at most 64 KB where eight of them hold the row, three CTAs to an SM; more parts where there are few rows
+        int ctas = 1;
+        while (ctas < 8 && (bytes > (size_t)ctas * 66 * 1024 || (p.rows * ctas < (size_t)ctx->sm_count * 2 && bytes / (ctas * 2) >= 4096))) ctas *= 2;
+        if (p.rows * ctas > 0x7fffffffull) return fail(ctx, PSSA_B200_ERR_SHAPE, "B200 distillation: too many rows; refusing launch");
+        return with_dtype(p.dtype, [&](auto t) { return launch_parts<decltype(t)>(ctx, p, ctas); });
+    }
     const size_t smem = ((size_t)p.vocab + 31) / 32 * 4;
     if (smem > 200 * 1024)
         return fail(ctx, PSSA_B200_ERR_UNSUPPORTED, "B200 distillation: vocabulary %d exceeds one CTA's marks; refusing launch", p.vocab);
     return with_dtype(p.dtype, [&](auto t) -> int32_t {
         static PerDeviceOnce attr;
-        if (smem > 32 * 1024 && attr.need(ctx->device)) {
-            PSSA_CUDA(ctx, cudaFuncSetAttribute(distill_topk_kernel<decltype(t)>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
+        if (attr.need(ctx->device)) {
+            PSSA_CUDA(ctx, cudaFuncSetAttribute(distill_topk_long_kernel<decltype(t)>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
             attr.done(ctx->device);
         }
-        distill_topk_kernel<decltype(t)><<<(unsigned)p.rows, kThreads, smem, ctx->stream>>>(p);
-        return after_launch(ctx, "distill_topk_kernel");
+        distill_topk_long_kernel<decltype(t)><<<(unsigned)p.rows, kThreads, smem, ctx->stream>>>(p);
+        return after_launch(ctx, "distill_topk_long_kernel");
     });
 }
 
