@@ -40,7 +40,7 @@ __device__ __forceinline__ T block_reduce(T v, T* scratch, F op) {
 template <typename T>
 __global__ void __launch_bounds__(kThreads) distill_topk_long_kernel(DistillParams p) {
     extern __shared__ unsigned s_bits[];
-    __shared__ float s_f[kWarps], s_x[PSSA_B200_MAX_TEACHER], s_t[PSSA_B200_MAX_TEACHER];
+    __shared__ float s_f[kWarps], s_t[PSSA_B200_MAX_TEACHER];
     __shared__ double s_d[kWarps];
     __shared__ unsigned s_u[kWarps], s_id[PSSA_B200_MAX_TEACHER];
     const size_t row = blockIdx.x;
@@ -77,9 +77,8 @@ __global__ void __launch_bounds__(kThreads) distill_topk_long_kernel(DistillPara
         t = st != 0.0f ? e / st : 0.0f;
         log_t = q - mt - logf(st);
     }
-    s_id[tid] = entry ? id : PSSA_B200_NO_TOKEN;
-    s_t[tid] = t;
-    s_x[tid] = entry ? to_f32(x[id]) : -INFINITY;
+    const float xe = entry ? to_f32(x[id]) : -INFINITY;
+    if (tid < PSSA_B200_MAX_TEACHER) s_id[tid] = entry ? id : PSSA_B200_NO_TOKEN, s_t[tid] = t;
     __syncthreads();
     bool first = entry;
     float t_at = 0.0f;
@@ -100,7 +99,7 @@ __global__ void __launch_bounds__(kThreads) distill_topk_long_kernel(DistillPara
     }
     su = block_reduce(su, s_f, sum);
     s1 = block_reduce(s1, s_f, sum);
-    const float z = empty ? -INFINITY : (s_x[tid] - m) * inv_t;
+    const float z = empty ? -INFINITY : (xe - m) * inv_t;
     const float s = su + block_reduce(first ? expf(z) : 0.0f, s_f, sum);
     const float ls = logf(s), log_rest = logf(su) - ls, p_rest = su / s;
     float term = t > 0.0f || t != t ? t * (log_t - (empty ? -INFINITY : z - ls)) : 0.0f;
@@ -144,22 +143,83 @@ __global__ void __launch_bounds__(kThreads) distill_topk_long_kernel(DistillPara
 struct RestSums {  // of a CTA's unlisted ids: sums at the temperature, and at 1
     float top, ref, sum, sum1;
 };
+struct Teacher {  // what one warp makes of a row's entries while the row is on its way
+    uint32_t id[PSSA_B200_MAX_TEACHER];  // PSSA_B200_NO_TOKEN: absent
+    float t[PSSA_B200_MAX_TEACHER], log_t[PSSA_B200_MAX_TEACHER], x[PSSA_B200_MAX_TEACHER];
+    float t_at[PSSA_B200_MAX_TEACHER];   // the id's whole mass at its first entry, -1 at others of it
+    float x_max, rest, mass;             // of the listed logits; 1 - sum t, with DISTILL_REST; sum t + rest
+    int bad, target;                     // a listed logit is no number; the target's entry or -1
+};
+
+// run by one warp; k entries in steps of 32
+template <typename T>
+__device__ void read_teacher(const DistillParams& p, size_t row, const T* x, uint32_t tgt, Teacher& s, bool report) {
+    const int lane = threadIdx.x & 31, v = p.vocab;
+    const float inv = 1.0f / p.teacher_temperature;
+    float q_max = -INFINITY, x_max = -INFINITY;
+    bool wrong = false, bad = false, any = false;
+    for (int i = lane; i < p.k; i += 32) {
+        const uint32_t id = p.teacher_ids[row * p.k + i];
+        const bool entry = id < (uint32_t)v;
+        const float q = entry ? p.teacher[row * p.k + i] * inv : -INFINITY, xe = entry ? to_f32(x[id]) : -INFINITY;
+        wrong |= !entry && id != PSSA_B200_NO_TOKEN;
+        any |= entry, bad |= xe != xe;
+        s.id[i] = entry ? id : PSSA_B200_NO_TOKEN, s.x[i] = xe, s.log_t[i] = q;
+        q_max = fmaxf(q_max, q != q ? INFINITY : q), x_max = fmaxf(x_max, xe);
+    }
+    if (report && wrong) atomicExch(p.status, PSSA_B200_ERR_TOKEN);
+    float rest = 0.0f, mass = 0.0f;
+    if (p.rest) {
+        double sum = 0.0;
+        for (int i = lane; i < p.k; i += 32) {
+            const float q = s.log_t[i];
+            s.t[i] = expf(q);
+            sum += exp((double)q);
+        }
+#pragma unroll
+        for (int m = 16; m > 0; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+        if (__any_sync(0xffffffffu, any)) rest = fmaxf((float)(1.0 - sum), 0.0f);  // no entry: nothing to learn
+    } else {
+        q_max = warp_max(q_max);  // infinite with a NaN, which then goes through the sum
+        float sum = 0.0f;
+        for (int i = lane; i < p.k; i += 32) {
+            const float e = q_max > -INFINITY ? expf(s.log_t[i] - q_max) : 0.0f;
+            s.t[i] = e, sum += e;
+        }
+        sum = warp_sum(sum);
+        const float log_sum = logf(sum);
+        for (int i = lane; i < p.k; i += 32) s.t[i] = sum != 0.0f ? s.t[i] / sum : 0.0f, s.log_t[i] = s.log_t[i] - q_max - log_sum;
+    }
+    for (int i = lane; i < p.k; i += 32) mass += s.t[i];
+    __syncwarp();
+    int target = -1;
+    for (int i = lane; i < p.k; i += 32) {
+        const uint32_t id = s.id[i];
+        float t_at = 0.0f;
+        bool first = id != PSSA_B200_NO_TOKEN;
+        if (first)
+            for (int j = 0; j < p.k; ++j)
+                if (s.id[j] == id) first = first && j >= i, t_at += s.t[j];
+        s.t_at[i] = first ? t_at : -1.0f;
+        if (first && id == tgt) target = i;
+    }
+    x_max = warp_max(x_max), mass = warp_sum(mass) + rest;
+    target = __reduce_max_sync(0xffffffffu, target), bad = __any_sync(0xffffffffu, bad);
+    if (lane == 0) s.x_max = x_max, s.rest = rest, s.mass = mass, s.bad = bad, s.target = target;
+}
 
 // A CTA holds elements [rank * each, + each) of a row, at the distance from a 16-byte boundary that they have in global memory.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) distill_topk_kernel(DistillParams p, int ctas, int each) {
     extern __shared__ __align__(128) unsigned char s_raw[];
-    __shared__ float s_f[kWarps], s_t[PSSA_B200_MAX_TEACHER];
-    __shared__ double s_d[kWarps];
-    __shared__ unsigned s_id[PSSA_B200_MAX_TEACHER];
+    __shared__ Teacher s_teacher;
+    __shared__ float s_top[kWarps], s_ref[kWarps], s_sum[kWarps], s_sum1[kWarps];
     __shared__ RestSums s_part;
     __shared__ __align__(8) uint64_t s_bar;
     constexpr int N = kVec<T>;
     const size_t row = blockIdx.x / (unsigned)ctas;
-    const int rank = blockIdx.x % (unsigned)ctas, tid = threadIdx.x, v = p.vocab;
+    const int rank = blockIdx.x % (unsigned)ctas, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, v = p.vocab;
     const T* x = static_cast<const T*>(p.logits) + row * p.ld;
-    auto sum = [](auto a, auto b) { return a + b; };
-    auto most = [](float a, float b) { return fmaxf(a, b); };
 
     // the part, on its way to shared memory: whole 16-byte pieces by one bulk copy, what lies around them by single loads
     const int e0 = min(rank * each, v), e1 = min(e0 + each, v), n = e1 - e0;
@@ -180,152 +240,166 @@ __global__ void __launch_bounds__(kThreads) distill_topk_kernel(DistillParams p,
     }
     if (tid < head) held[tid] = from[tid];
     if (tail0 + tid < n) held[tail0 + tid] = from[tail0 + tid];
-
-    // the teacher's entries, one to a thread
     const float inv_t = 1.0f / p.temperature, c = kLog2e / p.temperature;
-    const uint32_t id = tid < p.k ? p.teacher_ids[row * p.k + tid] : PSSA_B200_NO_TOKEN;
     const uint32_t tgt = p.targets ? p.targets[row] : PSSA_B200_NO_TOKEN;
-    const bool entry = id < (uint32_t)v, has = tgt < (uint32_t)v, none = tgt == PSSA_B200_NO_TOKEN;
+    const bool has = tgt < (uint32_t)v, none = tgt == PSSA_B200_NO_TOKEN;
+    if (warp == 0) read_teacher(p, row, x, has ? tgt : PSSA_B200_NO_TOKEN - 1, s_teacher, rank == 0);
     const float w_kl = p.grad_kl ? p.grad_kl[row] : 0.0f, w_ce = p.grad_ce && has ? p.grad_ce[row] : 0.0f;
-    const float xe = entry ? to_f32(x[id]) : -INFINITY, xt = has ? to_f32(x[tgt]) : -INFINITY;
-    const float q = entry ? p.teacher[row * p.k + tid] * (1.0f / p.teacher_temperature) : -INFINITY;
-    if (rank == 0 && ((!entry && id != PSSA_B200_NO_TOKEN) || (tid == 0 && !has && !none))) atomicExch(p.status, PSSA_B200_ERR_TOKEN);
-    float t, log_t = q, r = 0.0f;
-    if (p.rest) {
-        t = entry ? expf(q) : 0.0f;
-        r = fmaxf((float)(1.0 - block_reduce(entry ? exp((double)q) : 0.0, s_d, sum)), 0.0f);
-        if (!__syncthreads_or(entry)) r = 0.0f;  // no entry: nothing to learn
-    } else {
-        const float mt = block_reduce(entry && q != q ? INFINITY : q, s_f, most);  // a NaN goes through the sum
-        const float e = entry && mt > -INFINITY ? expf(q - mt) : 0.0f;
-        const float st = block_reduce(e, s_f, sum);
-        t = st != 0.0f ? e / st : 0.0f;
-        log_t = q - mt - logf(st);
+    float xt = -INFINITY;
+    if (tid == 0 && rank == 0) {
+        if (has) xt = to_f32(x[tgt]);
+        if (!has && !none) atomicExch(p.status, PSSA_B200_ERR_TOKEN);
     }
-    s_id[tid] = entry ? id : PSSA_B200_NO_TOKEN;
-    s_t[tid] = t;
-    __syncthreads();  // also: the barrier is ready for every thread
-    bool first = entry;  // of the entries with its id
-    float t_at = 0.0f;
-    if (entry)
-        for (int j = 0; j < p.k; ++j)
-            if (s_id[j] == id) {
-                first = first && j >= tid;
-                t_at += s_t[j];
-            }
+    __syncthreads();  // the entries, and the barrier
     if (vecs && !tc::mbar_wait(&s_bar, 0)) {
         atomicExch(p.status, PSSA_B200_ERR_TIMEOUT);
         tc::mbar_wait(&s_bar, 0);  // no CTA leaves with its copy on the way, if a wait can help it
     }
-    const bool mine = entry && id >= (uint32_t)e0 && id < (uint32_t)e1;
+    const uint32_t id = tid < p.k ? s_teacher.id[tid] : PSSA_B200_NO_TOKEN;
+    const bool mine = id >= (uint32_t)e0 && id < (uint32_t)e1;
     if (mine) held[id - e0] = from_f32<T>(-INFINITY);
     __syncthreads();
 
     // the sums of the ids that are not listed; at temperature 1 they serve the cross entropy too
     const bool two = p.targets && p.temperature != 1.0f;
     SoftmaxSums<false> rest, rest1;
-    for (int i = tid; i < vecs; i += kThreads) {
-        float f[N];
-        unpack<T>(held_vec[i], f);
-        rest.add(f, 0, c);
-        if (two) rest1.add(f, 0, kLog2e);
+    {
+        float f[N], m = -INFINITY;
+        if (tid < vecs) {
+            unpack<T>(held_vec[tid], f);
+            m = vector_max<T>(held_vec[tid], f);
+        }
+        m = warp_max(m);
+        rest.start(m, c), rest1.start(m, kLog2e);
     }
+    auto sweep = [&](auto both) {
+        for (int i = tid; i < vecs; i += kThreads) {
+            const uint4 raw = held_vec[i];
+            float f[N];
+            unpack<T>(raw, f);
+            const float m = vector_max<T>(raw, f);
+            rest.add(f, m, 0, c);
+            if (both) rest1.add(f, m, 0, kLog2e);
+        }
+    };
+    if (two)
+        sweep(std::true_type());
+    else
+        sweep(std::false_type());
     auto single = [&](int i) {
         const float f = to_f32(held[i]);
-        rest.add1(f, 0, c);
-        if (two) rest1.add1(f, 0, kLog2e);
+        rest.add1(f, c);
+        if (two) rest1.add1(f, kLog2e);
     };
     if (tid < head) single(tid);
     if (tail0 + tid < n) single(tail0 + tid);
-    const float p_ref = block_reduce(rest.ref, s_f, most), p_top = block_reduce(rest.top, s_f, most);
-    float part = rest.total(), part1 = rest1.total(), unused = 0.0f;
-    rebase(rest.ref, p_ref, c, part, unused);
-    rebase(rest1.ref, p_ref, kLog2e, part1, unused);
-    part = block_reduce(part, s_f, sum);
-    if (two) part1 = block_reduce(part1, s_f, sum);
-    if (tid == 0) s_part = RestSums{p_top, p_ref, part, two ? part1 : part};
-    const cg::cluster_group cluster = cg::this_cluster();
-    if (ctas > 1)
-        cluster.sync();
-    else
-        __syncthreads();
-    RestSums all = s_part;
-    if (ctas > 1) {
-        all = *cluster.map_shared_rank(&s_part, 0);
-        for (int i = 1; i < ctas; ++i) {
-            RestSums o = *cluster.map_shared_rank(&s_part, i);
-            const float to = fmaxf(all.ref, o.ref);
-            rebase(all.ref, to, c, all.sum, unused);
-            rebase(o.ref, to, c, o.sum, unused);
-            rebase(all.ref, to, kLog2e, all.sum1, unused);
-            rebase(o.ref, to, kLog2e, o.sum1, unused);
-            all.ref = to, all.top = fmaxf(all.top, o.top), all.sum += o.sum, all.sum1 += o.sum1;
+    {
+        const float ref = warp_max(fmaxf(rest.ref, rest1.ref)), top = warp_max(rest.top);
+        float sum = rest.total(), sum1 = rest1.total(), unused = 0.0f;
+        rebase(rest.ref, ref, c, sum, unused);
+        rebase(rest1.ref, ref, kLog2e, sum1, unused);
+        sum = warp_sum(sum);
+        if (two) sum1 = warp_sum(sum1);
+        if (lane == 0) s_top[warp] = top, s_ref[warp] = ref, s_sum[warp] = sum, s_sum1[warp] = two ? sum1 : sum;
+    }
+    __syncthreads();
+    auto join = [&](RestSums& a, RestSums b) {
+        const float to = fmaxf(a.ref, b.ref);
+        float unused = 0.0f;
+        rebase(a.ref, to, c, a.sum, unused);
+        rebase(b.ref, to, c, b.sum, unused);
+        if (two) {
+            rebase(a.ref, to, kLog2e, a.sum1, unused);
+            rebase(b.ref, to, kLog2e, b.sum1, unused);
         }
+        a.ref = to, a.top = fmaxf(a.top, b.top), a.sum += b.sum, a.sum1 += b.sum1;
+    };
+    RestSums all{s_top[0], s_ref[0], s_sum[0], s_sum1[0]};
+    for (int i = 1; i < kWarps; ++i) join(all, RestSums{s_top[i], s_ref[i], s_sum[i], s_sum1[i]});
+    const cg::cluster_group cluster = cg::this_cluster();
+    if (ctas > 1) {
+        if (tid == 0) s_part = all;
+        cluster.sync();  // and every CTA has read the listed logits: from here on their places may be written
+        all = *cluster.map_shared_rank(&s_part, 0);
+        for (int i = 1; i < ctas; ++i) join(all, *cluster.map_shared_rank(&s_part, i));
+        cluster.barrier_arrive();
     }
     // with the listed ids: everything relative to the row's maximum m, the rest's sum to its own
-    const float xe_max = block_reduce(xe, s_f, most), m = fmaxf(all.top, xe_max);
-    const bool bad = __syncthreads_or(xe != xe) || all.sum != all.sum || m == INFINITY, empty = m == -INFINITY;
-    const float z = empty ? -INFINITY : (xe - m) * inv_t;
+    const float m = fmaxf(all.top, s_teacher.x_max), r = s_teacher.rest, mass = s_teacher.mass;
+    const bool bad = s_teacher.bad || all.sum != all.sum || m == INFINITY, empty = m == -INFINITY;
     const float to_m = empty ? 0.0f : fmaxf(all.ref - m, -FLT_MAX);
-    const float s = all.sum * ex2(to_m * c) + block_reduce(first ? expf(z) : 0.0f, s_f, sum);
-    const float ls = logf(s);
+    auto z_of = [&](float a) { return empty ? -INFINITY : (a - m) * inv_t; };
+    float listed = 0.0f, listed1 = 0.0f;  // each warp for itself
+    for (int i = lane; i < p.k; i += 32)
+        if (s_teacher.t_at[i] >= 0.0f) {
+            listed += expf(z_of(s_teacher.x[i]));
+            if (two) listed1 += expf(empty ? -INFINITY : s_teacher.x[i] - m);
+        }
+    const float s = all.sum * ex2(to_m * c) + warp_sum(listed), ls = logf(s);
+    const float s1 = two ? all.sum1 * ex2(to_m * kLog2e) + warp_sum(listed1) : s;
     const float log_rest = to_m * inv_t + logf(all.sum) - ls, p_rest = expf(log_rest);
-    float s1 = s;
-    if (two) s1 = all.sum1 * ex2(to_m * kLog2e) + block_reduce(first ? expf(empty ? -INFINITY : xe - m) : 0.0f, s_f, sum);
-    const float mass = block_reduce(t, s_f, sum) + r;
-    if (rank == 0) {
-        const float term = t > 0.0f || t != t ? t * (log_t - (empty ? -INFINITY : z - ls)) : 0.0f;
-        float kl = block_reduce(term, s_f, sum);
+    if (rank == 0 && warp == 0) {
+        float kl = 0.0f;
+        for (int i = lane; i < p.k; i += 32) {
+            const float t = s_teacher.t[i];
+            if (t > 0.0f || t != t) kl += t * (s_teacher.log_t[i] - (empty ? -INFINITY : z_of(s_teacher.x[i]) - ls));
+        }
+        kl = warp_sum(kl);
         if (r > 0.0f) kl += r * (logf(r) - (empty || all.sum == 0.0f ? -INFINITY : log_rest));
-        if (tid == 0) {
+        if (lane == 0) {
             if (p.kl) p.kl[row] = bad ? kNan : kl;
             if (p.ce) p.ce[row] = none ? 0.0f : bad || !has ? kNan : empty ? INFINITY : logf(s1) - (xt - m);
         }
     }
-    if (ctas > 1) cluster.sync();  // the other CTAs' sums have been read, and all logits that lie where the gradient goes
-    if (!p.grad) return;
-    const bool zero = (w_kl == 0.0f && w_ce == 0.0f) || (empty && !bad);
-    const float g = w_kl * inv_t;
-    // an unlisted id: its share of the rest, times a, and its probability at temperature 1
-    const float a = all.sum > 0.0f ? g * (p.rest ? mass * p_rest - r : mass * p_rest) / all.sum : 0.0f;
-    const float a1 = w_ce * ex2(to_m * kLog2e) / s1;
-    const float both = two ? a : a + a1;
-    T* out = static_cast<T*>(p.grad) + row * p.ld_grad + e0;
-    const bool ce2 = two && w_ce != 0.0f;
-    auto grad = [&](float f) {
-        const float d = f - all.ref;
-        float y = both * ex2(d * c);
-        if (ce2) y = fmaf(a1, ex2(d * kLog2e), y);
-        return zero ? 0.0f : bad ? kNan : y;
-    };
-    const bool together = ((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(from)) & 15) == 0;
-    if (together) {
-        uint4* out_vec = reinterpret_cast<uint4*>(out + head);
-        for (int i = tid; i < vecs; i += kThreads) {
-            float f[N];
-            unpack<T>(held_vec[i], f);
+    if (p.grad) {
+        const bool zero = (w_kl == 0.0f && w_ce == 0.0f) || (empty && !bad);
+        const float g = w_kl * inv_t;
+        // an unlisted id: its share of the rest, times a, and its probability at temperature 1
+        const float a = all.sum > 0.0f ? g * (p.rest ? mass * p_rest - r : mass * p_rest) / all.sum : 0.0f;
+        const float a1 = w_ce * ex2(to_m * kLog2e) / s1, both = two ? a : a + a1;
+        const float nref = -all.ref;
+        T* out = static_cast<T*>(p.grad) + row * p.ld_grad + e0;
+        const bool together = ((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(from)) & 15) == 0;
+        auto write = [&](auto grad) {
+            if (together) {
+                uint4* out_vec = reinterpret_cast<uint4*>(out + head);
+                for (int i = tid; i < vecs; i += kThreads) {
+                    float f[N];
+                    unpack<T>(held_vec[i], f);
 #pragma unroll
-            for (int e = 0; e < N; ++e) f[e] = grad(f[e]);
-            out_vec[i] = pack<T>(f);
+                    for (int e = 0; e < N; ++e) f[e] = grad(f[e]);
+                    out_vec[i] = pack<T>(f);
+                }
+                if (tid < head) out[tid] = from_f32<T>(grad(to_f32(held[tid])));
+                if (tail0 + tid < n) out[tail0 + tid] = from_f32<T>(grad(to_f32(held[tail0 + tid])));
+            } else {
+                for (int i = tid; i < n; i += kThreads) out[i] = from_f32<T>(grad(to_f32(held[i])));
+            }
+        };
+        if (zero || bad) {
+            const float y = zero ? 0.0f : kNan;
+            write([&](float) { return y; });
+        } else {
+            auto one = [&](float f) { return both * ex2((f + nref) * c); };
+            auto with_ce = [&](float f) { return fmaf(a1, ex2((f + nref) * kLog2e), both * ex2((f + nref) * c)); };
+            const bool ce2 = two && w_ce != 0.0f;
+            if (ce2)
+                write(with_ce);
+            else
+                write(one);
+            const float xt_here = has && tgt >= (uint32_t)e0 && tgt < (uint32_t)e1 ? to_f32(held[tgt - e0]) : 0.0f;
+            __syncthreads();  // the listed ids and the target go over what has been written
+            if (mine && s_teacher.t_at[tid] >= 0.0f) {
+                const float xe = s_teacher.x[tid];
+                float d = g * (mass * (expf(z_of(xe)) / s) - s_teacher.t_at[tid]);
+                if (w_ce != 0.0f) d += w_ce * (expf(xe - m) / s1 - (id == tgt ? 1.0f : 0.0f));
+                out[id - e0] = from_f32<T>(d);
+            }
+            if (tid == 0 && w_ce != 0.0f && s_teacher.target < 0 && tgt >= (uint32_t)e0 && tgt < (uint32_t)e1)
+                out[tgt - e0] = from_f32<T>((ce2 ? with_ce(xt_here) : one(xt_here)) - w_ce);
         }
-        if (tid < head) out[tid] = from_f32<T>(grad(to_f32(held[tid])));
-        if (tail0 + tid < n) out[tail0 + tid] = from_f32<T>(grad(to_f32(held[tail0 + tid])));
-    } else {
-        for (int i = tid; i < n; i += kThreads) out[i] = from_f32<T>(grad(to_f32(held[i])));
     }
-    if (bad || zero) return;
-    __syncthreads();  // the listed ids and the target go over what has been written
-    bool at_target = false;
-    if (mine && first) {
-        float d = g * (mass * (expf(z) / s) - t_at);
-        if (w_ce != 0.0f) {
-            at_target = id == tgt;
-            d += w_ce * (expf(xe - m) / s1 - (at_target ? 1.0f : 0.0f));
-        }
-        out[id - e0] = from_f32<T>(d);
-    }
-    const bool listed = __syncthreads_or(entry && id == tgt);
-    if (tid == 0 && w_ce != 0.0f && !listed && tgt >= (uint32_t)e0 && tgt < (uint32_t)e1) out[tgt - e0] = from_f32<T>(grad(xt) - w_ce);
+    if (ctas > 1) cluster.barrier_wait();  // no CTA leaves while its sums are read
 }
 
 template <typename T>

@@ -172,19 +172,34 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LogprobParams p
     auto take = [&](uint4 raw, int at) {
         float f[N];
         unpack<T>(raw, f);
-        sums.add(f, part.head + at * N, c);
-        float m = f[0];
-#pragma unroll
-        for (int i = 1; i < N; ++i) m = fmaxf(m, f[i]);
+        const float m = vector_max<T>(raw, f);
+        sums.add(f, m, at, c);
         if (m > xt) {
 #pragma unroll
             for (int i = 0; i < N; ++i) above += f[i] > xt;
         }
     };
+    const int one = part.single();
+    const float single = one >= 0 ? to_f32(x[one]) : -INFINITY;
     int at = part.v0 + tid;
-    if (TOP) {  // until something is above -inf the lowest id of the share is its best
-        const int i = part.single();
-        sums.id = i >= 0 && i < part.head ? i : at < part.v1 ? part.head + at * N : i;
+    {
+        uint4 raw[kAhead];
+        float m = single;
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+            if (at + i * THREADS < part.v1) raw[i] = part.vec[at + i * THREADS];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+            if (at + i * THREADS < part.v1) {
+                float f[N];
+                unpack<T>(raw[i], f);
+                m = fmaxf(m, vector_max<T>(raw[i], f));
+            }
+        sums.start(warp_max(m), c);
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+            if (at + i * THREADS < part.v1) take(raw[i], at + i * THREADS);
+        at += kAhead * THREADS;
     }
     for (; at + (kAhead - 1) * THREADS < part.v1; at += kAhead * THREADS) {
         uint4 raw[kAhead];
@@ -194,12 +209,25 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LogprobParams p
         for (int i = 0; i < kAhead; ++i) take(raw[i], at + i * THREADS);
     }
     for (; at < part.v1; at += THREADS) take(part.vec[at], at);
-    if (const int i = part.single(); i >= 0) {
-        const float f = to_f32(x[i]);
-        // a head's ids are below, a tail's above all others of the thread: the lowest id of the best stays right
-        if (f == sums.top && i < sums.id) sums.id = i;
-        sums.add1(f, i, c);
-        above += f > xt;
+    Key own = 0;  // the thread's best logit
+    if (TOP) {
+        if (const int w = sums.where >= 0 ? sums.where : part.v0 + tid; w < part.v1) {  // without one above -inf, the lowest of its ids
+            float f[N];
+            unpack<T>(part.vec[w], f);
+            int e = 0;
+#pragma unroll
+            for (int i = N - 1; i >= 0; --i)
+                if (f[i] == sums.top) e = i;
+            own = key_of(sums.top, part.head + w * N + e);
+        }
+        if (one >= 0) {
+            const Key k = key_of(single, one);
+            own = k > own ? k : own;
+        }
+    }
+    if (one >= 0) {
+        sums.add1(single, c);
+        above += single > xt;
     }
     // the CTA's numbers
     const float ref = block_reduce<THREADS>(sums.ref, s.f[0], [](float a, float b) { return fmaxf(a, b); });
@@ -219,7 +247,7 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LogprobParams p
         for (int i = 0; i < kWarps; ++i) sum += s.f[1][i], ent += s.f[2][i], above += s.u[i];
         s.part = RowPart{top, ref, sum, ent, above};
     }
-    if (TOP) best_of_part<T, THREADS>(part, sums.id >= 0 ? key_of(sums.top, sums.id) : 0, p.top_n, s);
+    if (TOP) best_of_part<T, THREADS>(part, own, p.top_n, s);
     // the cluster's
     const cg::cluster_group cluster = cg::this_cluster();
     if (ctas > 1)
@@ -236,6 +264,7 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LogprobParams p
             all.ref = to, all.top = fmaxf(all.top, o.top), all.sum += o.sum, all.ent += o.ent, all.above += o.above;
         }
         const bool bad = all.sum != all.sum || all.top == INFINITY, empty = all.top == -INFINITY;
+        if (!empty) rebase(all.ref, all.top, c, all.sum, all.ent);
         const float ls = empty ? 0.0f : logf(all.sum);
         auto logp = [&](float a) { return bad ? kNan : empty ? -INFINITY : (a - all.top) * inv_t - ls; };
         if (tid == 0) {
