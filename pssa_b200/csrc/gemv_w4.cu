@@ -8,6 +8,7 @@
 #include "device_math.cuh"
 #include "element.cuh"
 #include "kernels.hpp"
+#include "logit_row.cuh"
 
 namespace pssa {
 namespace {
@@ -34,6 +35,7 @@ struct W4Split {
     int stage;       // of them in shared memory at a time
     int k_warps;     // warps of a CTA that share weight rows and split the columns
     int slice;       // input rows of a CTA
+    int group_chunks;  // of a group of 128 and more
     int vec;         // x starts and steps on 16 bytes
 };
 
@@ -155,7 +157,7 @@ __device__ __forceinline__ void stage_run(const T* x, size_t col, bool in, int v
 // A CTA: kWarps / k_warps warps side by side over weight rows, each with MT times 16 of them, times k_warps over the columns' chunks; up to NT times 8
 // columns of B. The CTAs of a cluster split the columns further; the first of them joins their sums. Sums are joined in a fixed order.
 template <typename T, int NT, int MT, int MODE>
-__global__ void __launch_bounds__(kThreads, 2) gemv_w4_kernel(GemvW4Params p, W4Split sp) {
+__global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) gemv_w4_kernel(GemvW4Params p, W4Split sp) {
     extern __shared__ uint4 s_x[];
     constexpr int P = Mma<T>::pieces;
     constexpr uint32_t kMagic = Mma<T>::magic;
@@ -168,18 +170,34 @@ __global__ void __launch_bounds__(kThreads, 2) gemv_w4_kernel(GemvW4Params p, W4
     const size_t row_bytes = p.w.k >> 1;
     const int k = (int)p.w.k;
 
-    // this lane's rows are n_lane + 8 m
+    // this lane's rows are n_lane + 8 m; it fetches the scales and zeros of the t-th of them, for its quad
     const size_t n_lane = n0 + (size_t)wm * MT * 16 + g;
     const int left = n_lane < p.w.n ? (int)min(p.w.n - n_lane, (size_t)MT * 16) : 0;
     const uint8_t* codes = p.w.codes + (left ? n_lane : 0) * row_bytes + 16 * t;
-    const size_t scale0 = (left ? n_lane : 0) * p.w.groups;
-    auto fetch = [&](int chunk, uint4 (&w)[2 * MT]) {
+    constexpr int kGroups = MODE == 0 ? 1 : 2 * MODE;  // of a chunk
+    const bool scaled = t < 2 * MT && 8 * t < left;
+    const size_t scale0 = scaled ? (n_lane + 8 * t) * p.w.groups : 0;
+    const int groups = scaled ? (int)p.w.groups : 0;
+    struct Fetched {
+        uint4 w[2 * MT];
+        float scale[kGroups];
+        uint32_t zero[kGroups];
+    };
+    auto fetch = [&](int chunk, Fetched& f) {
         const bool in = chunk < c1 && chunk * kChunk + 32 * t < k;
 #pragma unroll
-        for (int m = 0; m < 2 * MT; ++m) w[m] = in && 8 * m < left ? load_codes(codes + m * 8 * row_bytes + (size_t)chunk * (kChunk / 2)) : make_uint4(0, 0, 0, 0);
+        for (int m = 0; m < 2 * MT; ++m)
+            f.w[m] = in && 8 * m < left ? load_codes(codes + m * 8 * row_bytes + (size_t)chunk * (kChunk / 2)) : make_uint4(0, 0, 0, 0);
+        const int group0 = MODE != 0 ? chunk * kGroups : sp.group_chunks == 1 ? chunk : (int)((unsigned)chunk / (unsigned)sp.group_chunks);
+#pragma unroll
+        for (int q = 0; q < kGroups; ++q) {
+            const bool there = chunk < c1 && group0 + q < groups;
+            f.scale[q] = there ? load_f32(p.w.scales, p.w.scale_dtype, scale0 + group0 + q) : 0.0f;
+            if (p.w.zeros) f.zero[q] = there ? p.w.zeros[scale0 + group0 + q] : 0u;
+        }
     };
     float acc[MT][NT][4] = {};
-    uint4 now[2 * MT], next[2 * MT];
+    Fetched now, next;
     fetch(c0 + wk, now);
 
     const T* x = static_cast<const T*>(p.x) + r0 * p.ldx;
@@ -203,18 +221,15 @@ __global__ void __launch_bounds__(kThreads, 2) gemv_w4_kernel(GemvW4Params p, W4
         for (int chunk = first + wk; chunk < last; chunk += sp.k_warps) {
             fetch(chunk + sp.k_warps, next);
             const uint4* xs = s_x + b * buffer + (size_t)(chunk - first) * 16 * cols + lane;
-            constexpr int kGroups = MODE == 0 ? 1 : 2 * MODE;  // of a chunk
-            const size_t group0 = MODE == 0 ? (size_t)chunk * kChunk / p.w.group : (size_t)chunk * kGroups;
             float scale[2 * MT][kGroups];
             uint32_t zero[2 * MT][kGroups];
 #pragma unroll
             for (int m = 0; m < 2 * MT; ++m) {
-                by_group<MODE>(t, now[m]);
+                by_group<MODE>(t, now.w[m]);
 #pragma unroll
                 for (int q = 0; q < kGroups; ++q) {
-                    const bool in = 8 * m < left && (MODE == 0 || group0 + q < p.w.groups);
-                    scale[m][q] = in ? load_f32(p.w.scales, p.w.scale_dtype, scale0 + m * 8 * p.w.groups + group0 + q) : 0.0f;
-                    zero[m][q] = kMagic | (!p.w.zeros ? 0x00080008u : in ? (uint32_t)p.w.zeros[scale0 + m * 8 * p.w.groups + group0 + q] * 0x00010001u : 0u);
+                    scale[m][q] = __shfl_sync(0xffffffffu, now.scale[q], (lane & 28) + m);
+                    zero[m][q] = kMagic | (p.w.zeros ? __shfl_sync(0xffffffffu, now.zero[q], (lane & 28) + m) * 0x00010001u : 0x00080008u);
                 }
             }
             float part[MT][NT][4] = {};
@@ -225,7 +240,7 @@ __global__ void __launch_bounds__(kThreads, 2) gemv_w4_kernel(GemvW4Params p, W4
                 uint32_t a[MT][8];  // the word's registers of rows g and g + 8
 #pragma unroll
                 for (int m = 0; m < 2 * MT; ++m) {
-                    const uint32_t w = i == 0 ? now[m].x : i == 1 ? now[m].y : i == 2 ? now[m].z : now[m].w;
+                    const uint32_t w = i == 0 ? now.w[m].x : i == 1 ? now.w[m].y : i == 2 ? now.w[m].z : now.w[m].w;
 #pragma unroll
                     for (int j = 0; j < 4; ++j) a[m >> 1][2 * j + (m & 1)] = minus2<T>((w >> 4 * j & 0x000f000fu) | kMagic, zero[m][q]);
                 }
@@ -250,8 +265,7 @@ __global__ void __launch_bounds__(kThreads, 2) gemv_w4_kernel(GemvW4Params p, W4
                             }
                 }
             }
-#pragma unroll
-            for (int m = 0; m < 2 * MT; ++m) now[m] = next[m];
+            now = next;
         }
     }
     // the warps' sums side by side in shared memory, [k_warps][cta_rows][cols]
@@ -312,6 +326,82 @@ __device__ __forceinline__ void store_scale(void* scales, int dtype, size_t i, f
         static_cast<__half*>(scales)[i] = from_f32<__half>(v);
 }
 
+// Scale, zero and codes of one group that `LANES` neighbouring lanes hold 8 columns each of; the order of every fp32 operation is the definition's.
+struct GroupForm {
+    float step, inv, zero;
+    bool live;
+};
+template <int LANES>
+__device__ __forceinline__ GroupForm group_form(const W4Params& p, size_t at, float lo, float hi, bool bad, bool store) {
+#pragma unroll
+    for (int m = LANES / 2; m > 0; m >>= 1) {
+        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, m));
+        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, m));
+        bad |= __shfl_xor_sync(0xffffffffu, (int)bad, m) != 0;
+    }
+    float step = p.zeros ? __fdiv_rn(__fsub_rn(hi, lo), 15.0f) : __fdiv_rn(fmaxf(hi, -lo), 7.0f);
+    step = fminf(step, p.scale_dtype == PSSA_B200_F32 ? 3.402823466e38f : p.scale_dtype == PSSA_B200_BF16 ? 3.3895314e38f : 65504.0f);
+    if (bad) step = __builtin_nanf("");
+    if (store) store_scale(p.scales, p.scale_dtype, at, step);
+    if (p.scale_dtype == PSSA_B200_BF16) step = to_f32(from_f32<__nv_bfloat16>(step));
+    if (p.scale_dtype == PSSA_B200_F16) step = to_f32(from_f32<__half>(step));
+    GroupForm f;
+    f.step = step, f.live = step > 0.0f;
+    f.zero = !p.zeros ? 8.0f : f.live ? fminf(fmaxf(rintf(__fdiv_rn(-lo, step)), 0.0f), 15.0f) : 0.0f;
+    f.inv = 1.0f / step;
+    if (store && p.zeros) p.zeros[at] = (uint8_t)f.zero;
+    return f;
+}
+// clamp(rint(a / step) + zero, 0, 15). The product with 1 / step is within 3e-6 of the quotient where it is below 16, so that both round to the same whole number unless it
+// lies within 1e-5 of the middle of two; there, and where it is no number, the division decides. Above 16 both clamp.
+__device__ __forceinline__ unsigned code_of(const GroupForm& f, float a) {
+    const float v = a * f.inv;
+    float q = rintf(v);
+    if (!(fabsf(v - q) < 0.49999f)) q = rintf(__fdiv_rn(a, f.step));
+    return (unsigned)(f.live ? fminf(fmaxf(q + f.zero, 0.0f), 15.0f) : f.zero);
+}
+
+// Groups of LANES * 8 columns, 32 / LANES of them to a warp at a time and AHEAD times that on their way: one read of the weights, bound by it. A lane's 8 codes are
+// one word. w starts on 16 bytes.
+constexpr int kAhead = 4;
+template <typename T, int LANES>
+__global__ void __launch_bounds__(kThreads) w4_quantize_groups_kernel(W4Params p, const T* __restrict__ w) {
+    constexpr int kWords = 8 * sizeof(T) / 16;  // 16-byte words of 8 columns
+    const size_t total = p.n * p.groups, first = ((size_t)blockIdx.x * kThreads + threadIdx.x) / LANES, step = kThreads / LANES;
+    const size_t at0 = first + (size_t)blockIdx.x * step * (kAhead - 1);
+    const int lane = threadIdx.x % LANES;
+    uint4 raw[kAhead][kWords];
+    size_t off[kAhead];
+    bool in[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+        const size_t at = at0 + i * step, n = total >> 32 ? at / p.groups : (unsigned)at / (unsigned)p.groups, k = (at - n * p.groups) * p.group + 8 * lane;
+        in[i] = at < total && k < p.k, off[i] = n * p.k + k;
+#pragma unroll
+        for (int j = 0; j < kWords; ++j) raw[i][j] = in[i] ? reinterpret_cast<const uint4*>(w + off[i])[j] : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+        float x[8], lo = 0.0f, hi = 0.0f;
+        if constexpr (sizeof(T) == 4) {
+            unpack<T>(raw[i][0], *reinterpret_cast<float(*)[4]>(x));
+            unpack<T>(raw[i][1], *reinterpret_cast<float(*)[4]>(x + 4));
+        } else {
+            unpack<T>(raw[i][0], x);
+        }
+        bool bad = false;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) lo = fminf(lo, x[j]), hi = fmaxf(hi, x[j]), bad |= !isfinite(x[j]);
+        const size_t at = at0 + i * step;
+        const GroupForm f = group_form<LANES>(p, at, lo, hi, bad, lane == 0 && at < total);
+        unsigned word = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) word |= code_of(f, x[j]) << 4 * j;
+        if (in[i]) *reinterpret_cast<unsigned*>(p.codes + (off[i] >> 1)) = word;
+    }
+}
+
+// Groups of any length, one to a warp, read twice; and weights that start anywhere.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) w4_quantize_kernel(W4Params p, const T* __restrict__ w) {
     const size_t at = ((size_t)blockIdx.x * kThreads + threadIdx.x) >> 5;
@@ -325,41 +415,35 @@ __global__ void __launch_bounds__(kThreads) w4_quantize_kernel(W4Params p, const
         bad |= !isfinite(a);
         lo = fminf(lo, a), hi = fmaxf(hi, a);
     }
-#pragma unroll
-    for (int m = 16; m > 0; m >>= 1) {
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, m));
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, m));
-    }
-    bad = __any_sync(0xffffffffu, bad);
-    float step = p.zeros ? __fdiv_rn(__fsub_rn(hi, lo), 15.0f) : __fdiv_rn(fmaxf(hi, -lo), 7.0f);
-    step = fminf(step, p.scale_dtype == PSSA_B200_F32 ? 3.402823466e38f : p.scale_dtype == PSSA_B200_BF16 ? 3.3895314e38f : 65504.0f);
-    if (bad) step = __builtin_nanf("");
-    if (lane == 0) store_scale(p.scales, p.scale_dtype, at, step);
-    if (p.scale_dtype == PSSA_B200_BF16) step = to_f32(from_f32<__nv_bfloat16>(step));
-    if (p.scale_dtype == PSSA_B200_F16) step = to_f32(from_f32<__half>(step));
-    const bool live = step > 0.0f;
-    const float zero = !p.zeros ? 8.0f : live ? fminf(fmaxf(rintf(__fdiv_rn(-lo, step)), 0.0f), 15.0f) : 0.0f;
-    if (lane == 0 && p.zeros) p.zeros[at] = (uint8_t)zero;
+    const GroupForm f = group_form<32>(p, at, lo, hi, bad, lane == 0);
     for (size_t k = k0 + 2 * lane; k < k1; k += 64) {
-        unsigned byte = 0;
-        for (int j = 0; j < 2; ++j) {
-            const float a = to_f32(w[n * p.k + k + j]);
-            const float c = live ? fminf(fmaxf(rintf(__fdiv_rn(a, step)) + zero, 0.0f), 15.0f) : zero;
-            byte |= (unsigned)c << 4 * j;
-        }
-        p.codes[(n * p.k + k) >> 1] = (uint8_t)byte;
+        const unsigned even = code_of(f, to_f32(w[n * p.k + k])), odd = code_of(f, to_f32(w[n * p.k + k + 1]));
+        p.codes[(n * p.k + k) >> 1] = (uint8_t)(even | odd << 4);
     }
 }
 
 }  // namespace
 
 int32_t launch_w4_quantize(pssa_b200_ctx* ctx, const W4Params& w, const void* src, int dtype) {
-    const size_t blocks = (w.n * w.groups * 32 + kThreads - 1) / kThreads;
+    const bool together = w.group <= 256 && (reinterpret_cast<uintptr_t>(src) & 15) == 0;
+    const size_t lanes = together ? w.group / 8 : 32, per = kThreads / lanes * (together ? kAhead : 1), blocks = (w.n * w.groups + per - 1) / per;
     if (blocks > 0x7fffffff) return fail(ctx, PSSA_B200_ERR_SHAPE, "B200 4-bit weights: too many groups; refusing launch");
     with_dtype(dtype, [&](auto t) {
-        w4_quantize_kernel<<<(unsigned)blocks, kThreads, 0, ctx->stream>>>(w, static_cast<const decltype(t)*>(src));
+        using T = decltype(t);
+        const T* x = static_cast<const T*>(src);
+        const unsigned grid = (unsigned)blocks;
+        if (!together)
+            w4_quantize_kernel<<<grid, kThreads, 0, ctx->stream>>>(w, x);
+        else if (lanes == 4)
+            w4_quantize_groups_kernel<T, 4><<<grid, kThreads, 0, ctx->stream>>>(w, x);
+        else if (lanes == 8)
+            w4_quantize_groups_kernel<T, 8><<<grid, kThreads, 0, ctx->stream>>>(w, x);
+        else if (lanes == 16)
+            w4_quantize_groups_kernel<T, 16><<<grid, kThreads, 0, ctx->stream>>>(w, x);
+        else
+            w4_quantize_groups_kernel<T, 32><<<grid, kThreads, 0, ctx->stream>>>(w, x);
     });
-    return after_launch(ctx, "w4_quantize_kernel");
+    return after_launch(ctx, together ? "w4_quantize_groups_kernel" : "w4_quantize_kernel");
 }
 
 namespace {
@@ -368,6 +452,7 @@ int32_t launch_tiles(pssa_b200_ctx* ctx, const GemvW4Params& p) {
     constexpr int P = Mma<T>::pieces;
     W4Split sp{};
     sp.chunks = (int)((p.w.k + kChunk - 1) / kChunk);
+    sp.group_chunks = (int)(p.w.group / kChunk);
     sp.vec = (reinterpret_cast<uintptr_t>(p.x) & 15) == 0 && p.ldx * sizeof(T) % 16 == 0;
     sp.slice = (int)std::min<size_t>(p.rows, NT * 8 / P);
     sp.k_warps = NT >= 4 ? 2 : kWarps;

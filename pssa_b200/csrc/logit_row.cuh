@@ -2,6 +2,7 @@
 // cut of a row that starts anywhere into single elements and whole vectors.
 #pragma once
 #include <cfloat>
+#include <type_traits>
 
 #include "element.cuh"
 
