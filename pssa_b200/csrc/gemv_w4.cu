@@ -170,35 +170,45 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) gemv_w4_kernel(Gemv
     const size_t row_bytes = p.w.k >> 1;
     const int k = (int)p.w.k;
 
-    // this lane's rows are n_lane + 8 m; it fetches the scales and zeros of the t-th of them, for its quad
+    // This lane's weight rows are g + 8 m of the warp's; those behind the last row are not fetched, multiply what was there before and are not stored. It fetches the scales
+    // and zeros of the t-th of them, for its quad. Inputs behind the last column are staged as 0: any codes serve there.
     const size_t n_lane = n0 + (size_t)wm * MT * 16 + g;
     const int left = n_lane < p.w.n ? (int)min(p.w.n - n_lane, (size_t)MT * 16) : 0;
-    const uint8_t* codes = p.w.codes + (left ? n_lane : 0) * row_bytes + 16 * t;
+    const uint8_t* codes = p.w.codes + (left ? n_lane : 0) * row_bytes;
+    const size_t next_row = 8 * row_bytes;
+    const int last_word = (int)row_bytes - 16;
     constexpr int kGroups = MODE == 0 ? 1 : 2 * MODE;  // of a chunk
     const bool scaled = t < 2 * MT && 8 * t < left;
     const size_t scale0 = scaled ? (n_lane + 8 * t) * p.w.groups : 0;
     const int groups = scaled ? (int)p.w.groups : 0;
+    const bool wide = p.w.scale_dtype == PSSA_B200_F32;
     struct Fetched {
         uint4 w[2 * MT];
-        float scale[kGroups];
-        uint32_t zero[kGroups];
+        uint32_t scale[kGroups], zero[kGroups];  // as they lie
     };
     auto fetch = [&](int chunk, Fetched& f) {
-        const bool in = chunk < c1 && chunk * kChunk + 32 * t < k;
+        const uint8_t* at = codes + min(chunk * (kChunk / 2) + 16 * t, last_word);
 #pragma unroll
-        for (int m = 0; m < 2 * MT; ++m)
-            f.w[m] = in && 8 * m < left ? load_codes(codes + m * 8 * row_bytes + (size_t)chunk * (kChunk / 2)) : make_uint4(0, 0, 0, 0);
+        for (int m = 0; m < 2 * MT; ++m, at += next_row)
+            if (8 * m < left) f.w[m] = load_codes(at);
         const int group0 = MODE != 0 ? chunk * kGroups : sp.group_chunks == 1 ? chunk : (int)((unsigned)chunk / (unsigned)sp.group_chunks);
 #pragma unroll
         for (int q = 0; q < kGroups; ++q) {
-            const bool there = chunk < c1 && group0 + q < groups;
-            f.scale[q] = there ? load_f32(p.w.scales, p.w.scale_dtype, scale0 + group0 + q) : 0.0f;
-            if (p.w.zeros) f.zero[q] = there ? p.w.zeros[scale0 + group0 + q] : 0u;
+            const bool there = group0 + q < groups;
+            f.scale[q] = 0;
+            if (there) {
+                const size_t i = scale0 + group0 + q;
+                f.scale[q] = wide ? static_cast<const uint32_t*>(p.w.scales)[i] : static_cast<const uint16_t*>(p.w.scales)[i];
+                if (p.w.zeros) f.zero[q] = p.w.zeros[i];
+            }
         }
     };
     float acc[MT][NT][4] = {};
-    Fetched now, next;
-    fetch(c0 + wk, now);
+    Fetched now{}, next{};
+    if (c0 + wk < c1) fetch(c0 + wk, now);
+    int col_at[NT];  // this lane's place among a word's columns of B; the last column in place of those behind it, which are not stored
+#pragma unroll
+    for (int j = 0; j < NT; ++j) col_at[j] = min(j * 8 + g, cols - 1) * 4 + t;
 
     const T* x = static_cast<const T*>(p.x) + r0 * p.ldx;
     const int buffer = sp.stage * 16 * cols;  // 16-byte words of a stage
@@ -218,17 +228,22 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) gemv_w4_kernel(Gemv
         __syncthreads();
         const int last = min(first + sp.stage, c1);
         if (last < c1) stage(last, s_x + (b ^ 1) * buffer);
+#pragma unroll 2
         for (int chunk = first + wk; chunk < last; chunk += sp.k_warps) {
-            fetch(chunk + sp.k_warps, next);
-            const uint4* xs = s_x + b * buffer + (size_t)(chunk - first) * 16 * cols + lane;
-            float scale[2 * MT][kGroups];
+            if (chunk + sp.k_warps < c1) fetch(chunk + sp.k_warps, next);
+            const uint4* xs = s_x + b * buffer + (chunk - first) * 16 * cols;
+            float scale[2 * MT][kGroups], own[kGroups];
             uint32_t zero[2 * MT][kGroups];
+#pragma unroll
+            for (int q = 0; q < kGroups; ++q)
+                own[q] = wide ? __uint_as_float(now.scale[q]) : p.w.scale_dtype == PSSA_B200_BF16 ? __uint_as_float(now.scale[q] << 16) :
+                                                                __half2float(__ushort_as_half((unsigned short)now.scale[q]));
 #pragma unroll
             for (int m = 0; m < 2 * MT; ++m) {
                 by_group<MODE>(t, now.w[m]);
 #pragma unroll
                 for (int q = 0; q < kGroups; ++q) {
-                    scale[m][q] = __shfl_sync(0xffffffffu, now.scale[q], (lane & 28) + m);
+                    scale[m][q] = __shfl_sync(0xffffffffu, own[q], (lane & 28) + m);
                     zero[m][q] = kMagic | (p.w.zeros ? __shfl_sync(0xffffffffu, now.zero[q], (lane & 28) + m) * 0x00010001u : 0x00080008u);
                 }
             }
@@ -246,7 +261,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) gemv_w4_kernel(Gemv
                 }
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
-                    const uint4 v = j * 8 + g < cols ? xs[(i * cols + j * 8) * 4] : make_uint4(0, 0, 0, 0);
+                    const uint4 v = xs[i * cols * 4 + col_at[j]];
 #pragma unroll
                     for (int m = 0; m < MT; ++m) {
                         mma16816<T>(part[m][j], a[m][0], a[m][1], a[m][2], a[m][3], v.x, v.y);
@@ -326,9 +341,10 @@ __device__ __forceinline__ void store_scale(void* scales, int dtype, size_t i, f
         static_cast<__half*>(scales)[i] = from_f32<__half>(v);
 }
 
-// Scale, zero and codes of one group that `LANES` neighbouring lanes hold 8 columns each of; the order of every fp32 operation is the definition's.
+// Scale and zero of one group from its lanes' smallest and largest weight; the order of every fp32 operation is the definition's.
 struct GroupForm {
-    float step, inv, zero;
+    float step, inv;
+    int zero;
     bool live;
 };
 template <int LANES>
@@ -347,57 +363,84 @@ __device__ __forceinline__ GroupForm group_form(const W4Params& p, size_t at, fl
     if (p.scale_dtype == PSSA_B200_F16) step = to_f32(from_f32<__half>(step));
     GroupForm f;
     f.step = step, f.live = step > 0.0f;
-    f.zero = !p.zeros ? 8.0f : f.live ? fminf(fmaxf(rintf(__fdiv_rn(-lo, step)), 0.0f), 15.0f) : 0.0f;
-    f.inv = 1.0f / step;
+    f.zero = !p.zeros ? 8 : f.live ? (int)fminf(fmaxf(rintf(__fdiv_rn(-lo, step)), 0.0f), 15.0f) : 0;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(f.inv) : "f"(step));
     if (store && p.zeros) p.zeros[at] = (uint8_t)f.zero;
     return f;
 }
-// clamp(rint(a / step) + zero, 0, 15). The product with 1 / step is within 3e-6 of the quotient where it is below 16, so that both round to the same whole number unless it
-// lies within 1e-5 of the middle of two; there, and where it is no number, the division decides. Above 16 both clamp.
-__device__ __forceinline__ unsigned code_of(const GroupForm& f, float a) {
-    const float v = a * f.inv;
-    float q = rintf(v);
-    if (!(fabsf(v - q) < 0.49999f)) q = rintf(__fdiv_rn(a, f.step));
-    return (unsigned)(f.live ? fminf(fmaxf(q + f.zero, 0.0f), 15.0f) : f.zero);
+// clamp(rint(a / step) + zero, 0, 15)
+__device__ __noinline__ unsigned exact_code(float a, float step, int zero) {
+    return (unsigned)fminf(fmaxf(rintf(__fdiv_rn(a, step)) + (float)zero, 0.0f), 15.0f);
+}
+// The same for 8 weights, as one word. The product with 1 / step is within 3e-6 of the quotient where that is below 16, so that both round to the same whole
+// number unless it lies within 1e-5 of the middle of two; there, and where 1 / step is no number, the division decides, out of line. Adding 1.5 * 2^23 rounds to a
+// whole number and leaves it in the low bits: a conversion for each weight would be bound by the units that convert.
+__device__ __forceinline__ unsigned codes_of(const GroupForm& f, const float* x) {
+    if (!f.live) return 0x11111111u * (unsigned)f.zero;
+    constexpr float kRound = 12582912.0f;
+    float middle = f.inv >= FLT_MIN && f.inv <= FLT_MAX ? 0.0f : 1.0f;
+    unsigned word = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float v = fminf(fmaxf(x[j] * f.inv, -32.0f), 32.0f), r = v + kRound;
+        middle = fmaxf(middle, fabsf(v - (r - kRound)));
+        const int q = __float_as_int(r) - (__float_as_int(kRound) - f.zero);
+        word |= (unsigned)min(max(q, 0), 15) << 4 * j;
+    }
+    if (!(middle < 0.49999f)) {
+        word = 0;
+#pragma unroll 1
+        for (int j = 0; j < 8; ++j) {
+            float a = x[0];
+#pragma unroll
+            for (int i = 1; i < 8; ++i) a = i == j ? x[i] : a;
+            word |= exact_code(a, f.step, f.zero) << 4 * j;
+        }
+    }
+    return word;
 }
 
-// Groups of LANES * 8 columns, 32 / LANES of them to a warp at a time and AHEAD times that on their way: one read of the weights, bound by it. A lane's 8 codes are
-// one word. w starts on 16 bytes.
-constexpr int kAhead = 4;
+// Groups of LANES * 16 columns, 32 / LANES of them to a warp at a time and AHEAD times that on their way: one read of the weights. A lane's 16 codes are
+// 8 bytes. w starts on 16 bytes. 16384 x 8192 bf16 with zeros: 167 us with 8 columns a lane and a conversion a weight.
 template <typename T, int LANES>
 __global__ void __launch_bounds__(kThreads) w4_quantize_groups_kernel(W4Params p, const T* __restrict__ w) {
-    constexpr int kWords = 8 * sizeof(T) / 16;  // 16-byte words of 8 columns
-    const size_t total = p.n * p.groups, first = ((size_t)blockIdx.x * kThreads + threadIdx.x) / LANES, step = kThreads / LANES;
-    const size_t at0 = first + (size_t)blockIdx.x * step * (kAhead - 1);
+    constexpr int kWords = sizeof(T), kAhead = sizeof(T) == 4 ? 1 : 2;  // 16-byte words of 16 columns
+    const size_t total = p.n * p.groups, step = kThreads / LANES, at0 = (size_t)blockIdx.x * step * kAhead + threadIdx.x / LANES;
     const int lane = threadIdx.x % LANES;
     uint4 raw[kAhead][kWords];
     size_t off[kAhead];
     bool in[kAhead];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-        const size_t at = at0 + i * step, n = total >> 32 ? at / p.groups : (unsigned)at / (unsigned)p.groups, k = (at - n * p.groups) * p.group + 8 * lane;
+        const size_t at = at0 + i * step, n = total >> 32 ? at / p.groups : (unsigned)at / (unsigned)p.groups, k = (at - n * p.groups) * p.group + 16 * lane;
         in[i] = at < total && k < p.k, off[i] = n * p.k + k;
 #pragma unroll
         for (int j = 0; j < kWords; ++j) raw[i][j] = in[i] ? reinterpret_cast<const uint4*>(w + off[i])[j] : make_uint4(0, 0, 0, 0);
     }
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-        float x[8], lo = 0.0f, hi = 0.0f;
-        if constexpr (sizeof(T) == 4) {
-            unpack<T>(raw[i][0], *reinterpret_cast<float(*)[4]>(x));
-            unpack<T>(raw[i][1], *reinterpret_cast<float(*)[4]>(x + 4));
-        } else {
-            unpack<T>(raw[i][0], x);
-        }
+        float x[16], lo = 0.0f, hi = 0.0f;
         bool bad = false;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) lo = fminf(lo, x[j]), hi = fmaxf(hi, x[j]), bad |= !isfinite(x[j]);
+        for (int j = 0; j < kWords; ++j) unpack<T>(raw[i][j], *reinterpret_cast<float(*)[kVec<T>]>(x + j * kVec<T>));
+        if constexpr (sizeof(T) == 4) {
+            float none = 0.0f;  // a NaN once a weight is none or infinite
+#pragma unroll
+            for (int j = 0; j < 16; ++j) lo = fminf(lo, x[j]), hi = fmaxf(hi, x[j]), none = fmaf(x[j], 0.0f, none);
+            bad = none != none;
+        } else {  // two at a time, as they lie; a NaN stays one
+            using T2 = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+            const T2* h = reinterpret_cast<const T2*>(raw[i]);
+            T2 a = h[0], b = h[0];
+#pragma unroll
+            for (int j = 1; j < 8; ++j) a = __hmin2_nan(a, h[j]), b = __hmax2_nan(b, h[j]);
+            lo = fminf(to_f32(a.x), to_f32(a.y)), hi = fmaxf(to_f32(b.x), to_f32(b.y));
+            const float none = fmaf(to_f32(a.x), 0.0f, fmaf(to_f32(a.y), 0.0f, fmaf(to_f32(b.x), 0.0f, to_f32(b.y) * 0.0f)));
+            bad = none != none, lo = fminf(lo, 0.0f), hi = fmaxf(hi, 0.0f);
+        }
         const size_t at = at0 + i * step;
         const GroupForm f = group_form<LANES>(p, at, lo, hi, bad, lane == 0 && at < total);
-        unsigned word = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) word |= code_of(f, x[j]) << 4 * j;
-        if (in[i]) *reinterpret_cast<unsigned*>(p.codes + (off[i] >> 1)) = word;
+        if (in[i]) *reinterpret_cast<uint2*>(p.codes + (off[i] >> 1)) = make_uint2(codes_of(f, x), codes_of(f, x + 8));
     }
 }
 
@@ -417,7 +460,8 @@ __global__ void __launch_bounds__(kThreads) w4_quantize_kernel(W4Params p, const
     }
     const GroupForm f = group_form<32>(p, at, lo, hi, bad, lane == 0);
     for (size_t k = k0 + 2 * lane; k < k1; k += 64) {
-        const unsigned even = code_of(f, to_f32(w[n * p.k + k])), odd = code_of(f, to_f32(w[n * p.k + k + 1]));
+        const unsigned even = f.live ? exact_code(to_f32(w[n * p.k + k]), f.step, f.zero) : (unsigned)f.zero;
+        const unsigned odd = f.live ? exact_code(to_f32(w[n * p.k + k + 1]), f.step, f.zero) : (unsigned)f.zero;
         p.codes[(n * p.k + k) >> 1] = (uint8_t)(even | odd << 4);
     }
 }
@@ -425,8 +469,9 @@ __global__ void __launch_bounds__(kThreads) w4_quantize_kernel(W4Params p, const
 }  // namespace
 
 int32_t launch_w4_quantize(pssa_b200_ctx* ctx, const W4Params& w, const void* src, int dtype) {
-    const bool together = w.group <= 256 && (reinterpret_cast<uintptr_t>(src) & 15) == 0;
-    const size_t lanes = together ? w.group / 8 : 32, per = kThreads / lanes * (together ? kAhead : 1), blocks = (w.n * w.groups + per - 1) / per;
+    // lanes of a group share a warp evenly
+    const bool together = w.group <= 512 && (w.group & (w.group - 1)) == 0 && (reinterpret_cast<uintptr_t>(src) & 15) == 0;
+    const size_t lanes = together ? w.group / 16 : 32, per = kThreads / lanes * (together && dtype != PSSA_B200_F32 ? 2 : 1), blocks = (w.n * w.groups + per - 1) / per;
     if (blocks > 0x7fffffff) return fail(ctx, PSSA_B200_ERR_SHAPE, "B200 4-bit weights: too many groups; refusing launch");
     with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
@@ -434,6 +479,8 @@ int32_t launch_w4_quantize(pssa_b200_ctx* ctx, const W4Params& w, const void* sr
         const unsigned grid = (unsigned)blocks;
         if (!together)
             w4_quantize_kernel<<<grid, kThreads, 0, ctx->stream>>>(w, x);
+        else if (lanes == 2)
+            w4_quantize_groups_kernel<T, 2><<<grid, kThreads, 0, ctx->stream>>>(w, x);
         else if (lanes == 4)
             w4_quantize_groups_kernel<T, 4><<<grid, kThreads, 0, ctx->stream>>>(w, x);
         else if (lanes == 8)
