@@ -31,11 +31,13 @@ constexpr int kChunk = 128;
 
 struct W4Split {
     int chunks;      // of 128 columns
-    int per_cta;     // of them to a CTA of the cluster, which splits the columns
-    int stage;       // of them in shared memory at a time
+    int ctas;        // of a cluster, which splits the columns
+    int per_cta;     // chunks of a CTA
+    int stage;       // chunks whose inputs are in shared memory at a time
     int k_warps;     // warps of a CTA that share weight rows and split the columns
     int slice;       // input rows of a CTA
-    int group_chunks;  // of a group of 128 and more
+    int row_lots_log;  // of staging, see there
+    unsigned group_inverse;  // of a group's chunks: 2^32 over them, rounded up; 0 for one
     int vec;         // x starts and steps on 16 bytes
 };
 
@@ -66,14 +68,18 @@ __device__ __forceinline__ uint32_t minus2(uint32_t a, uint32_t b) {
     }
 }
 
-template <typename T>
-__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+// c (+)= a b; FIRST: without what c holds
+template <typename T, bool FIRST>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    const float c0 = FIRST ? 0.0f : c[0], c1 = FIRST ? 0.0f : c[1], c2 = FIRST ? 0.0f : c[2], c3 = FIRST ? 0.0f : c[3];
     if constexpr (std::is_same_v<T, __half>)
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
     else
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
 
 // word and lane that a chunk's run q of 8 columns ends up in
@@ -116,18 +122,18 @@ __device__ __forceinline__ uint4 interleave(uint4 v) {
     return make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
 }
 
-// columns [8 run, 8 run + 8) of an input row into place `at` (and, for fp32, the two after it in steps of `step`)
+// 8 inputs into place `at` (and, for fp32, the two after it in steps of `step`)
 template <typename T>
-__device__ __forceinline__ void stage_run(const T* x, size_t col, bool in, int vec, uint4* at, int step) {
+__device__ __forceinline__ void stage_run(const T* x, bool in, int vec, uint4* at, int step) {
     if constexpr (std::is_same_v<T, float>) {
         uint32_t u[8] = {};
         if (in) {
             if (vec) {
-                const uint4 a = *reinterpret_cast<const uint4*>(x + col), b = *reinterpret_cast<const uint4*>(x + col + 4);
+                const uint4 a = *reinterpret_cast<const uint4*>(x), b = *reinterpret_cast<const uint4*>(x + 4);
                 u[0] = a.x, u[1] = a.y, u[2] = a.z, u[3] = a.w, u[4] = b.x, u[5] = b.y, u[6] = b.z, u[7] = b.w;
             } else {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) u[j] = __float_as_uint(x[col + j]);
+                for (int j = 0; j < 8; ++j) u[j] = __float_as_uint(x[j]);
             }
         }
 #pragma unroll
@@ -143,9 +149,9 @@ __device__ __forceinline__ void stage_run(const T* x, size_t col, bool in, int v
         uint4 v = make_uint4(0, 0, 0, 0);
         if (in) {
             if (vec) {
-                v = *reinterpret_cast<const uint4*>(x + col);
+                v = *reinterpret_cast<const uint4*>(x);
             } else {
-                const uint16_t* h = reinterpret_cast<const uint16_t*>(x + col);
+                const uint16_t* h = reinterpret_cast<const uint16_t*>(x);
                 v = make_uint4(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16, h[4] | (uint32_t)h[5] << 16, h[6] | (uint32_t)h[7] << 16);
             }
         }
@@ -153,20 +159,36 @@ __device__ __forceinline__ void stage_run(const T* x, size_t col, bool in, int v
     }
 }
 
+__device__ __forceinline__ uint32_t masked(uint32_t w, uint32_t mask, uint32_t bits) {  // (w & mask) | bits
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(mask), "r"(bits));
+    return r;
+}
+// a word's codes of rows g and g + 8, less their zeros, as the A operands of two products: columns (0, 4), (1, 5) and (2, 6), (3, 7)
+template <typename T>
+__device__ __forceinline__ void numbers(uint32_t low, uint32_t high, uint32_t zero_low, uint32_t zero_high, uint32_t (&a)[2][4]) {
+    constexpr uint32_t kMagic = Mma<T>::magic;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        a[j >> 1][2 * (j & 1)] = minus2<T>(masked(low >> 4 * j, 0x000f000fu, kMagic), zero_low);
+        a[j >> 1][2 * (j & 1) + 1] = minus2<T>(masked(high >> 4 * j, 0x000f000fu, kMagic), zero_high);
+    }
+}
+
 // MODE 0: groups of 128 and more, 1: of 64, 2: of 32.
-// A CTA: kWarps / k_warps warps side by side over weight rows, each with MT times 16 of them, times k_warps over the columns' chunks; up to NT times 8
-// columns of B. The CTAs of a cluster split the columns further; the first of them joins their sums. Sums are joined in a fixed order.
+// A CTA: kWarps / k_warps warps side by side over weight rows, each with MT times 16 of them, times k_warps over the columns' chunks; NT times 8 columns of B. A warp has the
+// codes of its next chunk on their way while it multiplies one. The CTAs of a cluster split the columns further; the first of them joins their sums. Sums are joined in a fixed order.
 template <typename T, int NT, int MT, int MODE>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) gemv_w4_kernel(GemvW4Params p, W4Split sp) {
+__global__ void __launch_bounds__(kThreads, 2) gemv_w4_kernel(GemvW4Params p, W4Split sp) {
     extern __shared__ uint4 s_x[];
     constexpr int P = Mma<T>::pieces;
     constexpr uint32_t kMagic = Mma<T>::magic;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int wk = warp % sp.k_warps, wm = warp / sp.k_warps, m_warps = kWarps / sp.k_warps;
-    const int cta_rows = m_warps * MT * 16;
-    const size_t n0 = (size_t)blockIdx.y * cta_rows, r0 = (size_t)blockIdx.z * sp.slice;
+    const int cta_rows = m_warps * MT * 16, rank = blockIdx.x % (unsigned)sp.ctas;
+    const size_t n0 = (size_t)(blockIdx.x / (unsigned)sp.ctas) * cta_rows, r0 = (size_t)blockIdx.y * sp.slice;
     const int in_rows = (int)min((size_t)sp.slice, p.rows - r0), cols = in_rows * P;
-    const int c0 = min((int)blockIdx.x * sp.per_cta, sp.chunks), c1 = min(c0 + sp.per_cta, sp.chunks);
+    const int c0 = min(rank * sp.per_cta, sp.chunks), c1 = min(c0 + sp.per_cta, sp.chunks);
     const size_t row_bytes = p.w.k >> 1;
     const int k = (int)p.w.k;
 
@@ -181,7 +203,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) gemv_w4_kernel(Gemv
     const bool scaled = t < 2 * MT && 8 * t < left;
     const size_t scale0 = scaled ? (n_lane + 8 * t) * p.w.groups : 0;
     const int groups = scaled ? (int)p.w.groups : 0;
-    const bool wide = p.w.scale_dtype == PSSA_B200_F32;
+    const bool wide = p.w.scale_dtype == PSSA_B200_F32, halves = p.w.scale_dtype == PSSA_B200_F16;
+    const int scale_shift = wide ? 0 : 16;
     struct Fetched {
         uint4 w[2 * MT];
         uint32_t scale[kGroups], zero[kGroups];  // as they lie
@@ -191,16 +214,15 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) gemv_w4_kernel(Gemv
 #pragma unroll
         for (int m = 0; m < 2 * MT; ++m, at += next_row)
             if (8 * m < left) f.w[m] = load_codes(at);
-        const int group0 = MODE != 0 ? chunk * kGroups : sp.group_chunks == 1 ? chunk : (int)((unsigned)chunk / (unsigned)sp.group_chunks);
+        const int group0 = MODE != 0 ? chunk * kGroups : sp.group_inverse ? (int)__umulhi((unsigned)chunk, sp.group_inverse) : chunk;
 #pragma unroll
         for (int q = 0; q < kGroups; ++q) {
             const bool there = group0 + q < groups;
-            f.scale[q] = 0;
-            if (there) {
-                const size_t i = scale0 + group0 + q;
-                f.scale[q] = wide ? static_cast<const uint32_t*>(p.w.scales)[i] : static_cast<const uint16_t*>(p.w.scales)[i];
-                if (p.w.zeros) f.zero[q] = p.w.zeros[i];
-            }
+            const size_t i = scale0 + group0 + q;
+            f.scale[q] = 0, f.zero[q] = 8;
+            if (there && wide) f.scale[q] = static_cast<const uint32_t*>(p.w.scales)[i];
+            if (there && !wide) f.scale[q] = static_cast<const uint16_t*>(p.w.scales)[i];
+            if (there && p.w.zeros) f.zero[q] = p.w.zeros[i];
         }
     };
     float acc[MT][NT][4] = {};
@@ -211,75 +233,75 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) gemv_w4_kernel(Gemv
     for (int j = 0; j < NT; ++j) col_at[j] = min(j * 8 + g, cols - 1) * 4 + t;
 
     const T* x = static_cast<const T*>(p.x) + r0 * p.ldx;
-    const int buffer = sp.stage * 16 * cols;  // 16-byte words of a stage
-    auto stage = [&](int first, uint4* to) {
-        const int runs = (min(first + sp.stage, c1) - first) * 16;
-        for (int i = threadIdx.x; i < runs * in_rows; i += kThreads) {
-            const int r = i / runs, run = i - r * runs;
-            int word, at;
-            place<MODE>(run & 15, &word, &at);
-            const size_t col = (size_t)first * kChunk + 8 * run;
-            stage_run(x + (size_t)r * p.ldx, col, col < (size_t)k, sp.vec, to + (((run >> 4) * 4 + word) * cols + r * P) * 4 + at, 4);
+    // 16 threads to a chunk's runs of one row; the others take other rows, or chunks where there are few rows
+    const int run = threadIdx.x & 15, lot = threadIdx.x >> 4, row_lots = 1 << sp.row_lots_log, chunk_lots = kThreads / 16 >> sp.row_lots_log;
+    int run_word, run_at;
+    place<MODE>(run, &run_word, &run_at);
+    auto stage = [&](int first) {
+        const int last = min(first + sp.stage, c1);
+        for (int c = first + (lot >> sp.row_lots_log); c < last; c += chunk_lots) {
+            const int col = c * kChunk + 8 * run, r = lot & (row_lots - 1);
+            const T* from = x + (size_t)r * p.ldx + col;
+            uint4* at = s_x + (((c - first) * 4 + run_word) * cols + r * P) * 4 + run_at;
+#pragma unroll 2
+            for (int i = r; i < in_rows; i += row_lots, from += row_lots * p.ldx, at += row_lots * P * 4) stage_run(from, col < k, sp.vec, at, 4);
         }
     };
-    if (c0 < c1) stage(c0, s_x);
-    int b = 0;
-    for (int first = c0; first < c1; first += sp.stage, b ^= 1) {
-        __syncthreads();
-        const int last = min(first + sp.stage, c1);
-        if (last < c1) stage(last, s_x + (b ^ 1) * buffer);
-#pragma unroll 2
-        for (int chunk = first + wk; chunk < last; chunk += sp.k_warps) {
-            if (chunk + sp.k_warps < c1) fetch(chunk + sp.k_warps, next);
-            const uint4* xs = s_x + b * buffer + (chunk - first) * 16 * cols;
-            float scale[2 * MT][kGroups], own[kGroups];
-            uint32_t zero[2 * MT][kGroups];
+    auto work = [&](Fetched& f, const uint4* xs) {
 #pragma unroll
-            for (int q = 0; q < kGroups; ++q)
-                own[q] = wide ? __uint_as_float(now.scale[q]) : p.w.scale_dtype == PSSA_B200_BF16 ? __uint_as_float(now.scale[q] << 16) :
-                                                                __half2float(__ushort_as_half((unsigned short)now.scale[q]));
+        for (int m = 0; m < 2 * MT; ++m) by_group<MODE>(t, f.w[m]);
+        float part[MT][NT][4], own[kGroups];
+        uint32_t zero[2 * MT];
 #pragma unroll
-            for (int m = 0; m < 2 * MT; ++m) {
-                by_group<MODE>(t, now.w[m]);
+        for (int q = 0; q < kGroups; ++q) {
+            // fp32 and bf16 scales by a shift, fp16 ones converted: a choice of two numbers, not of two ways
+            const float shifted = __uint_as_float(f.scale[q] << scale_shift), half = __half2float(__ushort_as_half((unsigned short)f.scale[q]));
+            own[q] = halves ? half : shifted;
+        }
 #pragma unroll
-                for (int q = 0; q < kGroups; ++q) {
-                    scale[m][q] = __shfl_sync(0xffffffffu, own[q], (lane & 28) + m);
-                    zero[m][q] = kMagic | (p.w.zeros ? __shfl_sync(0xffffffffu, now.zero[q], (lane & 28) + m) * 0x00010001u : 0x00080008u);
-                }
+        for (int i = 0; i < 4; ++i) {
+            constexpr int kWords = 4 / kGroups;  // of a group
+            const int q = i / kWords;
+            if (i % kWords == 0) {
+#pragma unroll
+                for (int m = 0; m < 2 * MT; ++m) zero[m] = kMagic | __shfl_sync(0xffffffffu, f.zero[q], (lane & 28) + m) * 0x00010001u;
             }
-            float part[MT][NT][4] = {};
+            uint4 v[NT];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                constexpr int kWords = 4 / kGroups;  // of a group
-                const int q = i / kWords;
-                uint32_t a[MT][8];  // the word's registers of rows g and g + 8
+            for (int j = 0; j < NT; ++j) v[j] = xs[i * cols * 4 + col_at[j]];
 #pragma unroll
-                for (int m = 0; m < 2 * MT; ++m) {
-                    const uint32_t w = i == 0 ? now.w[m].x : i == 1 ? now.w[m].y : i == 2 ? now.w[m].z : now.w[m].w;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) a[m >> 1][2 * j + (m & 1)] = minus2<T>((w >> 4 * j & 0x000f000fu) | kMagic, zero[m][q]);
-                }
+            for (int m = 0; m < MT; ++m) {
+                auto word = [&](const uint4& w) { return i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w; };
+                uint32_t a[2][4];
+                numbers<T>(word(f.w[2 * m]), word(f.w[2 * m + 1]), zero[2 * m], zero[2 * m + 1], a);
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
-                    const uint4 v = xs[i * cols * 4 + col_at[j]];
-#pragma unroll
-                    for (int m = 0; m < MT; ++m) {
-                        mma16816<T>(part[m][j], a[m][0], a[m][1], a[m][2], a[m][3], v.x, v.y);
-                        mma16816<T>(part[m][j], a[m][4], a[m][5], a[m][6], a[m][7], v.z, v.w);
-                    }
+                    if (i % kWords == 0)
+                        mma16816<T, true>(part[m][j], a[0], v[j].x, v[j].y);
+                    else
+                        mma16816<T, false>(part[m][j], a[0], v[j].x, v[j].y);
                 }
+#pragma unroll
+                for (int j = 0; j < NT; ++j) mma16816<T, false>(part[m][j], a[1], v[j].z, v[j].w);
                 if ((i + 1) % kWords == 0) {  // a group's sums, or a chunk's of a longer group, meet their scale
+                    const float low = __shfl_sync(0xffffffffu, own[q], (lane & 28) + 2 * m), high = __shfl_sync(0xffffffffu, own[q], (lane & 28) + 2 * m + 1);
 #pragma unroll
                     for (int j = 0; j < NT; ++j)
 #pragma unroll
-                        for (int m = 0; m < MT; ++m)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                acc[m][j][e] = fmaf(part[m][j][e], scale[2 * m + (e >> 1)][q], acc[m][j][e]);
-                                part[m][j][e] = 0.0f;
-                            }
+                        for (int e = 0; e < 4; ++e) acc[m][j][e] = fmaf(part[m][j][e], e < 2 ? low : high, acc[m][j][e]);
                 }
             }
+        }
+    };
+    for (int first = c0; first < c1; first += sp.stage) {
+        if (first != c0) __syncthreads();
+        stage(first);
+        __syncthreads();
+        const int last = min(first + sp.stage, c1);
+#pragma unroll 2
+        for (int chunk = first + wk; chunk < last; chunk += sp.k_warps) {
+            if (chunk + sp.k_warps < c1) fetch(chunk + sp.k_warps, next);
+            work(now, s_x + (chunk - first) * 16 * cols);
             now = next;
         }
     }
@@ -299,8 +321,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) gemv_w4_kernel(Gemv
     __syncthreads();
     namespace cg = cooperative_groups;
     const cg::cluster_group cluster = cg::this_cluster();
-    const int ctas = gridDim.x;
-    if (ctas > 1) {
+    if (sp.ctas > 1) {
         for (int i = threadIdx.x; i < tile; i += kThreads) {
             float v = red[i];
             for (int w = 1; w < sp.k_warps; ++w) v += red[w * tile + i];
@@ -308,28 +329,27 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) gemv_w4_kernel(Gemv
         }
         cluster.sync();
     }
-    if (blockIdx.x == 0) {
-        T* out = static_cast<T*>(p.out) + r0 * p.ldo;
-        for (int i = threadIdx.x; i < cta_rows * in_rows; i += kThreads) {
-            const int r = i / cta_rows, row = i - r * cta_rows;
-            const size_t n = n0 + row;
-            if (n >= p.w.n) continue;
-            float v = 0.0f;
+    // each CTA of a cluster stores a part of the rows
+    const int each = cta_rows / sp.ctas;
+    T* out = static_cast<T*>(p.out) + r0 * p.ldo;
+    for (int i = threadIdx.x; i < each * in_rows; i += kThreads) {
+        const int r = i / each, row = rank * each + i - r * each;
+        const size_t n = n0 + row;
+        if (n >= p.w.n) continue;
+        float v = 0.0f;
 #pragma unroll
-            for (int piece = 0; piece < P; ++piece) {
-                const int at = row * cols + r * P + piece;
-                float u = red[at];
-                if (ctas > 1)
-                    for (int c = 1; c < ctas; ++c) u += cluster.map_shared_rank(red, c)[at];
-                else
-                    for (int w = 1; w < sp.k_warps; ++w) u += red[w * tile + at];
-                v = piece == 0 ? u : v + u;
-            }
-            T* o = out + (size_t)r * p.ldo + n;
-            *o = from_f32<T>(apply_epilogue(p.epilogue, v, p.alpha, p.epilogue == EPI_ADD_OUT ? to_f32(*o) : 0.0f));
+        for (int piece = 0; piece < P; ++piece) {
+            const int at = row * cols + r * P + piece;
+            float u[8] = {};
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+                if (sp.ctas > 1 ? c < sp.ctas : c < sp.k_warps) u[c] = sp.ctas > 1 ? cluster.map_shared_rank(red, c)[at] : red[c * tile + at];
+            v += ((u[0] + u[1]) + (u[2] + u[3])) + ((u[4] + u[5]) + (u[6] + u[7]));
         }
+        T* o = out + (size_t)r * p.ldo + n;
+        *o = from_f32<T>(apply_epilogue(p.epilogue, v, p.alpha, p.epilogue == EPI_ADD_OUT ? to_f32(*o) : 0.0f));
     }
-    if (ctas > 1) cluster.sync();  // no CTA leaves while its sums are read
+    if (sp.ctas > 1) cluster.sync();  // no CTA leaves while its sums are read
 }
 
 __device__ __forceinline__ void store_scale(void* scales, int dtype, size_t i, float v) {
@@ -495,30 +515,35 @@ int32_t launch_w4_quantize(pssa_b200_ctx* ctx, const W4Params& w, const void* sr
 
 namespace {
 template <typename T, int NT, int MT, int MODE>
-int32_t launch_tiles(pssa_b200_ctx* ctx, const GemvW4Params& p) {
+int32_t launch_tiles(pssa_b200_ctx* ctx, const GemvW4Params& p, int slice) {
     constexpr int P = Mma<T>::pieces;
     W4Split sp{};
     sp.chunks = (int)((p.w.k + kChunk - 1) / kChunk);
-    sp.group_chunks = (int)(p.w.group / kChunk);
+    // chunk * inverse >> 32 is chunk / group chunks while chunk * (group chunks) < 2^32
+    const size_t group_chunks = p.w.group / kChunk;
+    sp.group_inverse = group_chunks > 1 ? (unsigned)(((1ull << 32) + group_chunks - 1) / group_chunks) : 0;
+    if (sp.chunks > 65535) return fail(ctx, PSSA_B200_ERR_UNSUPPORTED, "B200 4-bit product: width %zu above 8388480; refusing launch", p.w.k);
     sp.vec = (reinterpret_cast<uintptr_t>(p.x) & 15) == 0 && p.ldx * sizeof(T) % 16 == 0;
-    sp.slice = (int)std::min<size_t>(p.rows, NT * 8 / P);
-    sp.k_warps = NT >= 4 ? 2 : kWarps;
+    sp.slice = slice;
+    while (1 << sp.row_lots_log < slice && sp.row_lots_log < 4) ++sp.row_lots_log;
+    const char* env = getenv("W4_KW");
+    sp.k_warps = env ? atoi(env) : NT <= 2 ? 8 : 1;
     const int cta_rows = kWarps / sp.k_warps * MT * 16;
-    const size_t tiles = (p.w.n + cta_rows - 1) / cta_rows, slices = (p.rows + sp.slice - 1) / sp.slice;
-    if (tiles > 65535 || slices > 65535) return fail(ctx, PSSA_B200_ERR_SHAPE, "B200 4-bit product: too many rows; refusing launch");
+    const size_t tiles = (p.w.n + cta_rows - 1) / cta_rows, slices = (p.rows + slice - 1) / slice;
+    if (tiles > 0x7fffffff / 8 || slices > 65535) return fail(ctx, PSSA_B200_ERR_SHAPE, "B200 4-bit product: too many rows; refusing launch");
     int ctas = 1;
     while (ctas < 8 && tiles * slices * ctas * 2 <= (size_t)ctx->sm_count * 2 && ctas * 2 * sp.k_warps <= sp.chunks) ctas *= 2;
-    sp.per_cta = (sp.chunks + ctas - 1) / ctas;
-    const size_t chunk_bytes = (size_t)16 * 16 * sp.slice * P, room = 48 * 1024;
+    sp.ctas = ctas, sp.per_cta = (sp.chunks + ctas - 1) / ctas;
+    const size_t chunk_bytes = (size_t)256 * slice * P, room = 96 * 1024;  // two CTAs to an SM
     sp.stage = (int)std::min<size_t>(sp.per_cta, std::max<size_t>(sp.k_warps, room / chunk_bytes / sp.k_warps * sp.k_warps));
-    const size_t smem = std::max(chunk_bytes * sp.stage * (sp.stage < sp.per_cta ? 2 : 1), (size_t)sp.k_warps * cta_rows * sp.slice * P * 4);
+    const size_t smem = std::max(chunk_bytes * sp.stage, (size_t)kWarps * MT * 16 * slice * P * 4);
     static PerDeviceOnce attr;
     if (attr.need(ctx->device)) {
         PSSA_CUDA(ctx, cudaFuncSetAttribute(gemv_w4_kernel<T, NT, MT, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
         attr.done(ctx->device);
     }
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(ctas, (unsigned)tiles, (unsigned)slices), cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = smem, cfg.stream = ctx->stream;
+    cfg.gridDim = dim3((unsigned)(tiles * ctas), (unsigned)slices), cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = smem, cfg.stream = ctx->stream;
     cudaLaunchAttribute at{};
     at.id = cudaLaunchAttributeClusterDimension;
     at.val.clusterDim.x = ctas, at.val.clusterDim.y = 1, at.val.clusterDim.z = 1;
@@ -531,13 +556,16 @@ int32_t launch_tiles(pssa_b200_ctx* ctx, const GemvW4Params& p) {
 int32_t launch_gemv_w4(pssa_b200_ctx* ctx, const GemvW4Params& p) {
     return with_dtype(p.dtype, [&](auto t) -> int32_t {
         using T = decltype(t);
+        constexpr size_t P = Mma<T>::pieces;
+        // up to 48 columns of B at a time, the rows spread evenly over as many times as that takes
+        const size_t most = std::min(p.rows, 48 / P), slices = (p.rows + most - 1) / most, slice = (p.rows + slices - 1) / slices, cols = slice * P;
         auto by_group = [&](auto mode) {
             constexpr int M = decltype(mode)::value;
-            const size_t cols = p.rows * Mma<T>::pieces;
-            if (cols <= 8) return launch_tiles<T, 1, 2, M>(ctx, p);
-            if (cols <= 16) return launch_tiles<T, 2, 2, M>(ctx, p);
-            if (cols <= 32) return launch_tiles<T, 4, 1, M>(ctx, p);
-            return launch_tiles<T, 8, 1, M>(ctx, p);
+            if (cols <= 8) return launch_tiles<T, 1, 2, M>(ctx, p, (int)slice);
+            if (cols <= 16) return launch_tiles<T, 2, 2, M>(ctx, p, (int)slice);
+            if (cols <= 24) return launch_tiles<T, 3, 1, M>(ctx, p, (int)slice);
+            if (cols <= 32) return launch_tiles<T, 4, 1, M>(ctx, p, (int)slice);
+            return launch_tiles<T, 6, 1, M>(ctx, p, (int)slice);
         };
         if (p.w.group == 32) return by_group(std::integral_constant<int, 2>());
         if (p.w.group == 64) return by_group(std::integral_constant<int, 1>());
