@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(kThreads, 2) gemv_w4_kernel(GemvW4Params p, W4
             const int col = c * kChunk + 8 * run, r = lot & (row_lots - 1);
             const T* from = x + (size_t)r * p.ldx + col;
             uint4* at = s_x + (((c - first) * 4 + run_word) * cols + r * P) * 4 + run_at;
-#pragma unroll 2
+#pragma unroll 6
             for (int i = r; i < in_rows; i += row_lots, from += row_lots * p.ldx, at += row_lots * P * 4) stage_run(from, col < k, sp.vec, at, 4);
         }
     };
@@ -332,6 +332,7 @@ __global__ void __launch_bounds__(kThreads, 2) gemv_w4_kernel(GemvW4Params p, W4
     // each CTA of a cluster stores a part of the rows
     const int each = cta_rows / sp.ctas;
     T* out = static_cast<T*>(p.out) + r0 * p.ldo;
+#pragma unroll 4
     for (int i = threadIdx.x; i < each * in_rows; i += kThreads) {
         const int r = i / each, row = rank * each + i - r * each;
         const size_t n = n0 + row;
@@ -526,8 +527,11 @@ int32_t launch_tiles(pssa_b200_ctx* ctx, const GemvW4Params& p, int slice) {
     sp.vec = (reinterpret_cast<uintptr_t>(p.x) & 15) == 0 && p.ldx * sizeof(T) % 16 == 0;
     sp.slice = slice;
     while (1 << sp.row_lots_log < slice && sp.row_lots_log < 4) ++sp.row_lots_log;
-    const char* env = getenv("W4_KW");
-    sp.k_warps = env ? atoi(env) : NT <= 2 ? 8 : 1;
+    // Warps take columns rather than rows while the GPU has room for the CTAs, two to an SM (head of 16384 x 768, 1 row: 6.8, 6.2, 5.7 and 7.5 us with 1, 2, 4 and 8 of
+    // them to a row). With many columns of B they share the staged inputs instead (48 rows of 16384 x 4096: 47, 57, 81 and 124 us).
+    sp.k_warps = 1;
+    while (NT <= 2 && sp.k_warps < kWarps && sp.k_warps < sp.chunks && (p.w.n * sp.k_warps * 2 + kWarps * MT * 16 - 1) / (kWarps * MT * 16) <= (size_t)ctx->sm_count * 2)
+        sp.k_warps *= 2;
     const int cta_rows = kWarps / sp.k_warps * MT * 16;
     const size_t tiles = (p.w.n + cta_rows - 1) / cta_rows, slices = (p.rows + slice - 1) / slice;
     if (tiles > 0x7fffffff / 8 || slices > 65535) return fail(ctx, PSSA_B200_ERR_SHAPE, "B200 4-bit product: too many rows; refusing launch");
