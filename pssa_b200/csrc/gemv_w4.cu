@@ -24,7 +24,7 @@ constexpr int kThreads = 256;
 // A chunk is 128 columns. Lane (g, t) of a warp (g = lane / 4, t = lane % 4) loads 16 bytes, 32 codes, of rows g and g + 8, so that a row's chunk
 // is 64 bytes in a row. Which columns the four lanes of a row multiply at a time is free as long as A and B agree, but all of one product have
 // to be of one group: as they lie for groups of 128 and more, after one exchange between lanes two apart for 64, after a 4 x 4
-// transposition for 32. `place` says where a run of 8 columns ends up. A word's 8 codes become 4 registers of two columns 4 apart, by a mask and the bits
+// transposition for 32. `run_placed` says which run of 8 columns is where. A word's 8 codes become 4 registers of two columns 4 apart, by a mask and the bits
 // of 128 (fp16: 1024) that put a code into a mantissa; x is staged with its runs in that order.
 constexpr int kWarps = kThreads / 32;
 constexpr int kChunk = 128;
@@ -82,15 +82,12 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
 
-// word and lane that a chunk's run q of 8 columns ends up in
+// the run of a chunk, of 8 columns, that ends up in a word of lane t
 template <int MODE>
-__device__ __forceinline__ void place(int q, int* word, int* t) {
-    if (MODE == 0)
-        *t = q >> 2, *word = q & 3;
-    else if (MODE == 2)
-        *word = q >> 2, *t = q & 3;
-    else
-        *word = (q & 1) + 2 * (q >> 3), *t = (q >> 2 & 1) + 2 * (q >> 1 & 1);
+__device__ __forceinline__ int run_placed(int word, int t) {
+    if (MODE == 0) return 4 * t + word;
+    if (MODE == 2) return 4 * word + t;
+    return (word & 1) + 8 * (word >> 1) + 4 * (t & 1) + 2 * (t >> 1);
 }
 
 __device__ __forceinline__ void swap_words(uint32_t& lo, uint32_t& hi, bool upper, int mask) {
@@ -122,42 +119,43 @@ __device__ __forceinline__ uint4 interleave(uint4 v) {
     return make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
 }
 
-// 8 inputs into place `at` (and, for fp32, the two after it in steps of `step`)
+// 8 inputs, as they lie
 template <typename T>
-__device__ __forceinline__ void stage_run(const T* x, bool in, int vec, uint4* at, int step) {
-    if constexpr (std::is_same_v<T, float>) {
-        uint32_t u[8] = {};
-        if (in) {
-            if (vec) {
-                const uint4 a = *reinterpret_cast<const uint4*>(x), b = *reinterpret_cast<const uint4*>(x + 4);
-                u[0] = a.x, u[1] = a.y, u[2] = a.z, u[3] = a.w, u[4] = b.x, u[5] = b.y, u[6] = b.z, u[7] = b.w;
-            } else {
+struct Run {
+    uint4 v[sizeof(T) / 2];
+    __device__ __forceinline__ void load(const T* x, bool in, int vec) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) u[j] = __float_as_uint(x[j]);
-            }
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = make_uint4(0, 0, 0, 0);
+        if (!in) return;
+        if (vec) {
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = reinterpret_cast<const uint4*>(x)[i];
+        } else if constexpr (sizeof(T) == 4) {
+            const uint32_t* u = reinterpret_cast<const uint32_t*>(x);
+            v[0] = make_uint4(u[0], u[1], u[2], u[3]), v[1] = make_uint4(u[4], u[5], u[6], u[7]);
+        } else {
+            const uint16_t* h = reinterpret_cast<const uint16_t*>(x);
+            v[0] = make_uint4(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16, h[4] | (uint32_t)h[5] << 16, h[6] | (uint32_t)h[7] << 16);
         }
-#pragma unroll
-        for (int piece = 0; piece < 3; ++piece) {
-            uint32_t o[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) o[j] = __byte_perm(u[j], u[j + 4], 0x7632);  // the upper halves: cut, not rounded
-            at[piece * step] = make_uint4(o[0], o[1], o[2], o[3]);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) u[j] = __float_as_uint(__uint_as_float(u[j]) - __uint_as_float(u[j] & 0xffff0000u));
-        }
-    } else {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (in) {
-            if (vec) {
-                v = *reinterpret_cast<const uint4*>(x);
-            } else {
-                const uint16_t* h = reinterpret_cast<const uint16_t*>(x);
-                v = make_uint4(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16, h[4] | (uint32_t)h[5] << 16, h[6] | (uint32_t)h[7] << 16);
-            }
-        }
-        *at = interleave(v);
     }
-}
+    // into place `at` in the order of the codes' registers, and for fp32 the two after it in steps of `step`
+    __device__ __forceinline__ void store(uint4* at, int step) const {
+        if constexpr (sizeof(T) == 4) {
+            uint32_t u[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w};
+#pragma unroll
+            for (int piece = 0; piece < 3; ++piece) {
+                uint32_t o[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[j] = __byte_perm(u[j], u[j + 4], 0x7632);  // the upper halves: cut, not rounded
+                at[piece * step] = make_uint4(o[0], o[1], o[2], o[3]);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) u[j] = __float_as_uint(__uint_as_float(u[j]) - __uint_as_float(u[j] & 0xffff0000u));
+            }
+        } else {
+            *at = interleave(v[0]);
+        }
+    }
+};
 
 __device__ __forceinline__ uint32_t masked(uint32_t w, uint32_t mask, uint32_t bits) {  // (w & mask) | bits
     uint32_t r;
@@ -175,11 +173,14 @@ __device__ __forceinline__ void numbers(uint32_t low, uint32_t high, uint32_t ze
     }
 }
 
+constexpr int ctas_per_sm(int nt) { return nt <= 2 ? 2 : 1; }
+constexpr int kMaxCols = 48;  // of B at a time
+
 // MODE 0: groups of 128 and more, 1: of 64, 2: of 32.
 // A CTA: kWarps / k_warps warps side by side over weight rows, each with MT times 16 of them, times k_warps over the columns' chunks; NT times 8 columns of B. A warp has the
 // codes of its next chunk on their way while it multiplies one. The CTAs of a cluster split the columns further; the first of them joins their sums. Sums are joined in a fixed order.
 template <typename T, int NT, int MT, int MODE>
-__global__ void __launch_bounds__(kThreads, 2) gemv_w4_kernel(GemvW4Params p, W4Split sp) {
+__global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) gemv_w4_kernel(GemvW4Params p, W4Split sp) {
     extern __shared__ uint4 s_x[];
     constexpr int P = Mma<T>::pieces;
     constexpr uint32_t kMagic = Mma<T>::magic;
@@ -233,19 +234,34 @@ __global__ void __launch_bounds__(kThreads, 2) gemv_w4_kernel(GemvW4Params p, W4
     for (int j = 0; j < NT; ++j) col_at[j] = min(j * 8 + g, cols - 1) * 4 + t;
 
     const T* x = static_cast<const T*>(p.x) + r0 * p.ldx;
-    // 16 threads to a chunk's runs of one row; the others take other rows, or chunks where there are few rows
-    const int run = threadIdx.x & 15, lot = threadIdx.x >> 4, row_lots = 1 << sp.row_lots_log, chunk_lots = kThreads / 16 >> sp.row_lots_log;
-    int run_word, run_at;
-    place<MODE>(run, &run_word, &run_at);
+    // 16 threads to a chunk's runs of one row; the others take other rows, or chunks where there are few rows. Lanes next to each other store to different banks.
+    const int run_at = threadIdx.x & 3, run_word = threadIdx.x >> 3 & 3, lot = (threadIdx.x >> 5) * 2 + (threadIdx.x >> 2 & 1);
+    const int run = run_placed<MODE>(run_word, run_at), row_lots = 1 << sp.row_lots_log, chunk_lots = kThreads / 16 >> sp.row_lots_log;
     auto stage = [&](int first) {
         const int last = min(first + sp.stage, c1);
-        for (int c = first + (lot >> sp.row_lots_log); c < last; c += chunk_lots) {
-            const int col = c * kChunk + 8 * run, r = lot & (row_lots - 1);
-            const T* from = x + (size_t)r * p.ldx + col;
-            uint4* at = s_x + (((c - first) * 4 + run_word) * cols + r * P) * 4 + run_at;
-#pragma unroll 6
-            for (int i = r; i < in_rows; i += row_lots, from += row_lots * p.ldx, at += row_lots * P * 4) stage_run(from, col < k, sp.vec, at, 4);
+        for (int r = lot & (row_lots - 1); r < in_rows; r += row_lots) {
+            const T* from = x + (size_t)r * p.ldx + 8 * run;
+            uint4* at = s_x + (run_word * cols + r * P) * 4 + run_at;
+#pragma unroll 4
+            for (int c = first + (lot >> sp.row_lots_log); c < last; c += chunk_lots) {
+                Run<T> v;
+                v.load(from + c * kChunk, c * kChunk + 8 * run < k, sp.vec);
+                v.store(at + (c - first) * 16 * cols, 4);
+            }
         }
+    };
+    // with many columns of B a chunk at a time: its inputs are on their way while the one before is multiplied
+    constexpr int kRuns = (kMaxCols / P * 16 + kThreads - 1) / kThreads;
+    Run<T> coming[kRuns];
+    auto load_chunk = [&](int c) {
+#pragma unroll
+        for (int u = 0; u < kRuns; ++u)
+            if (lot + 16 * u < in_rows) coming[u].load(x + (size_t)(lot + 16 * u) * p.ldx + c * kChunk + 8 * run, c * kChunk + 8 * run < k, sp.vec);
+    };
+    auto store_chunk = [&](uint4* to) {
+#pragma unroll
+        for (int u = 0; u < kRuns; ++u)
+            if (lot + 16 * u < in_rows) coming[u].store(to + (run_word * cols + (lot + 16 * u) * P) * 4 + run_at, 4);
     };
     auto work = [&](Fetched& f, const uint4* xs) {
 #pragma unroll
@@ -293,22 +309,40 @@ __global__ void __launch_bounds__(kThreads, 2) gemv_w4_kernel(GemvW4Params p, W4
             }
         }
     };
-    for (int first = c0; first < c1; first += sp.stage) {
-        if (first != c0) __syncthreads();
-        stage(first);
+    if constexpr (NT >= 3) {
+        if (c0 < c1) {
+            load_chunk(c0);
+            store_chunk(s_x);
+            if (c0 + 1 < c1) load_chunk(c0 + 1);
+        }
         __syncthreads();
-        const int last = min(first + sp.stage, c1);
 #pragma unroll 2
-        for (int chunk = first + wk; chunk < last; chunk += sp.k_warps) {
-            if (chunk + sp.k_warps < c1) fetch(chunk + sp.k_warps, next);
-            work(now, s_x + (chunk - first) * 16 * cols);
+        for (int c = c0; c < c1; ++c) {
+            if (c + 1 < c1) fetch(c + 1, next);
+            work(now, s_x + (c - c0 & 1) * 16 * cols);
+            if (c + 1 < c1) store_chunk(s_x + (c + 1 - c0 & 1) * 16 * cols);
+            if (c + 2 < c1) load_chunk(c + 2);
             now = next;
+            __syncthreads();
+        }
+    } else {
+        for (int first = c0; first < c1; first += sp.stage) {
+            if (first != c0) __syncthreads();
+            stage(first);
+            __syncthreads();
+            const int last = min(first + sp.stage, c1);
+#pragma unroll 2
+            for (int chunk = first + wk; chunk < last; chunk += sp.k_warps) {
+                if (chunk + sp.k_warps < c1) fetch(chunk + sp.k_warps, next);
+                work(now, s_x + (chunk - first) * 16 * cols);
+                now = next;
+            }
         }
     }
-    // the warps' sums side by side in shared memory, [k_warps][cta_rows][cols]
+    // the warps' sums side by side in shared memory, [k_warps][cta_rows][pitch]
     __syncthreads();
     float* red = reinterpret_cast<float*>(s_x);
-    const int tile = cta_rows * cols;
+    const int pitch = cols | 1, tile = cta_rows * pitch;  // odd: neighbouring rows in different banks
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -316,39 +350,42 @@ __global__ void __launch_bounds__(kThreads, 2) gemv_w4_kernel(GemvW4Params p, W4
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int row = (wm * MT + m) * 16 + (e >> 1) * 8 + g, col = j * 8 + 2 * t + (e & 1);
-                if (col < cols) red[wk * tile + row * cols + col] = acc[m][j][e];
+                if (col < cols) red[wk * tile + row * pitch + col] = acc[m][j][e];
             }
-    __syncthreads();
     namespace cg = cooperative_groups;
     const cg::cluster_group cluster = cg::this_cluster();
-    if (sp.ctas > 1) {
-        for (int i = threadIdx.x; i < tile; i += kThreads) {
-            float v = red[i];
-            for (int w = 1; w < sp.k_warps; ++w) v += red[w * tile + i];
-            red[i] = v;
-        }
+    if (sp.ctas > 1)
         cluster.sync();
-    }
-    // each CTA of a cluster stores a part of the rows
-    const int each = cta_rows / sp.ctas;
-    T* out = static_cast<T*>(p.out) + r0 * p.ldo;
-#pragma unroll 4
-    for (int i = threadIdx.x; i < each * in_rows; i += kThreads) {
-        const int r = i / each, row = rank * each + i - r * each;
-        const size_t n = n0 + row;
-        if (n >= p.w.n) continue;
-        float v = 0.0f;
+    else
+        __syncthreads();
+    // each CTA of a cluster joins and stores a part of the rows: neighbouring threads neighbouring rows of weights
+    const int each = cta_rows / sp.ctas, row = rank * each + threadIdx.x % each;
+    const size_t n = n0 + row;
+    if (n < p.w.n) {
+        T* out = static_cast<T*>(p.out) + r0 * p.ldo + n;
+#pragma unroll 2
+        for (int r = threadIdx.x / each; r < in_rows; r += kThreads / each) {
+            float v = 0.0f;
 #pragma unroll
-        for (int piece = 0; piece < P; ++piece) {
-            const int at = row * cols + r * P + piece;
-            float u[8] = {};
+            for (int piece = 0; piece < P; ++piece) {
+                const int at = row * pitch + r * P + piece;
+                float sum = 0.0f;
+                for (int c = 0; c < sp.ctas; ++c) {
+                    const float* from = sp.ctas > 1 ? cluster.map_shared_rank(red, c) : red;
+                    if constexpr (NT >= 3) {
+                        sum += from[at];
+                    } else {
+                        float u[kWarps];
 #pragma unroll
-            for (int c = 0; c < 8; ++c)
-                if (sp.ctas > 1 ? c < sp.ctas : c < sp.k_warps) u[c] = sp.ctas > 1 ? cluster.map_shared_rank(red, c)[at] : red[c * tile + at];
-            v += ((u[0] + u[1]) + (u[2] + u[3])) + ((u[4] + u[5]) + (u[6] + u[7]));
+                        for (int w = 0; w < kWarps; ++w) u[w] = w < sp.k_warps ? from[w * tile + at] : 0.0f;
+                        sum += ((u[0] + u[1]) + (u[2] + u[3])) + ((u[4] + u[5]) + (u[6] + u[7]));
+                    }
+                }
+                v += sum;
+            }
+            T* o = out + (size_t)r * p.ldo;
+            *o = from_f32<T>(apply_epilogue(p.epilogue, v, p.alpha, p.epilogue == EPI_ADD_OUT ? to_f32(*o) : 0.0f));
         }
-        T* o = out + (size_t)r * p.ldo + n;
-        *o = from_f32<T>(apply_epilogue(p.epilogue, v, p.alpha, p.epilogue == EPI_ADD_OUT ? to_f32(*o) : 0.0f));
     }
     if (sp.ctas > 1) cluster.sync();  // no CTA leaves while its sums are read
 }
@@ -536,11 +573,11 @@ int32_t launch_tiles(pssa_b200_ctx* ctx, const GemvW4Params& p, int slice) {
     const size_t tiles = (p.w.n + cta_rows - 1) / cta_rows, slices = (p.rows + slice - 1) / slice;
     if (tiles > 0x7fffffff / 8 || slices > 65535) return fail(ctx, PSSA_B200_ERR_SHAPE, "B200 4-bit product: too many rows; refusing launch");
     int ctas = 1;
-    while (ctas < 8 && tiles * slices * ctas * 2 <= (size_t)ctx->sm_count * 2 && ctas * 2 * sp.k_warps <= sp.chunks) ctas *= 2;
+    while (ctas < 8 && tiles * slices * ctas * 2 <= (size_t)ctx->sm_count * ctas_per_sm(NT) && ctas * 2 * sp.k_warps <= sp.chunks) ctas *= 2;
     sp.ctas = ctas, sp.per_cta = (sp.chunks + ctas - 1) / ctas;
     const size_t chunk_bytes = (size_t)256 * slice * P, room = 96 * 1024;  // two CTAs to an SM
-    sp.stage = (int)std::min<size_t>(sp.per_cta, std::max<size_t>(sp.k_warps, room / chunk_bytes / sp.k_warps * sp.k_warps));
-    const size_t smem = std::max(chunk_bytes * sp.stage, (size_t)kWarps * MT * 16 * slice * P * 4);
+    sp.stage = NT >= 3 ? 2 : (int)std::min<size_t>(sp.per_cta, std::max<size_t>(sp.k_warps, room / chunk_bytes / sp.k_warps * sp.k_warps));
+    const size_t smem = std::max(chunk_bytes * sp.stage, (size_t)kWarps * MT * 16 * (slice * P | 1) * 4);
     static PerDeviceOnce attr;
     if (attr.need(ctx->device)) {
         PSSA_CUDA(ctx, cudaFuncSetAttribute(gemv_w4_kernel<T, NT, MT, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
@@ -562,14 +599,14 @@ int32_t launch_gemv_w4(pssa_b200_ctx* ctx, const GemvW4Params& p) {
         using T = decltype(t);
         constexpr size_t P = Mma<T>::pieces;
         // up to 48 columns of B at a time, the rows spread evenly over as many times as that takes
-        const size_t most = std::min(p.rows, 48 / P), slices = (p.rows + most - 1) / most, slice = (p.rows + slices - 1) / slices, cols = slice * P;
+        const size_t most = std::min(p.rows, kMaxCols / P), slices = (p.rows + most - 1) / most, slice = (p.rows + slices - 1) / slices, cols = slice * P;
         auto by_group = [&](auto mode) {
             constexpr int M = decltype(mode)::value;
             if (cols <= 8) return launch_tiles<T, 1, 2, M>(ctx, p, (int)slice);
             if (cols <= 16) return launch_tiles<T, 2, 2, M>(ctx, p, (int)slice);
-            if (cols <= 24) return launch_tiles<T, 3, 1, M>(ctx, p, (int)slice);
-            if (cols <= 32) return launch_tiles<T, 4, 1, M>(ctx, p, (int)slice);
-            return launch_tiles<T, 6, 1, M>(ctx, p, (int)slice);
+            if (cols <= 24) return launch_tiles<T, 3, 2, M>(ctx, p, (int)slice);
+            if (cols <= 32) return launch_tiles<T, 4, 2, M>(ctx, p, (int)slice);
+            return launch_tiles<T, 6, 2, M>(ctx, p, (int)slice);
         };
         if (p.w.group == 32) return by_group(std::integral_constant<int, 2>());
         if (p.w.group == 64) return by_group(std::integral_constant<int, 1>());
