@@ -416,7 +416,7 @@ int32_t launch_parts(pssa_b200_ctx* ctx, const DistillParams& p, int ctas) {
     cudaLaunchAttribute at{};
     at.id = cudaLaunchAttributeClusterDimension;
     at.val.clusterDim.x = ctas, at.val.clusterDim.y = 1, at.val.clusterDim.z = 1;
-    cfg.attrs = &at, cfg.numAttrs = 1;
+    cfg.attrs = &at, cfg.numAttrs = ctas > 1;  // a launch with a cluster takes the host longer
     PSSA_CUDA(ctx, cudaLaunchKernelEx(&cfg, distill_topk_kernel<T>, p, ctas, (int)each));
     return after_launch(ctx, "distill_topk_kernel");
 }

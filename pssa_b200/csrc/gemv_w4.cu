@@ -588,7 +588,7 @@ int32_t launch_tiles(pssa_b200_ctx* ctx, const GemvW4Params& p, int slice) {
     cudaLaunchAttribute at{};
     at.id = cudaLaunchAttributeClusterDimension;
     at.val.clusterDim.x = ctas, at.val.clusterDim.y = 1, at.val.clusterDim.z = 1;
-    cfg.attrs = &at, cfg.numAttrs = 1;
+    cfg.attrs = &at, cfg.numAttrs = ctas > 1;  // a launch with a cluster takes the host longer
     PSSA_CUDA(ctx, cudaLaunchKernelEx(&cfg, gemv_w4_kernel<T, NT, MT, MODE>, p, sp));
     return after_launch(ctx, "gemv_w4_kernel");
 }

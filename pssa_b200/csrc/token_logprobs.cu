@@ -376,7 +376,7 @@ cudaError_t launch_rows(pssa_b200_ctx* ctx, const LogprobParams& p, int ctas) {
     cudaLaunchAttribute at{};
     at.id = cudaLaunchAttributeClusterDimension;
     at.val.clusterDim.x = ctas, at.val.clusterDim.y = 1, at.val.clusterDim.z = 1;
-    cfg.attrs = &at, cfg.numAttrs = 1;
+    cfg.attrs = &at, cfg.numAttrs = ctas > 1;  // a launch with a cluster takes the host longer
     return cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, THREADS, TOP>, p, ctas);
 }
 

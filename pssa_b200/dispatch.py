@@ -24,6 +24,14 @@ def _ptr(x):
     raise TypeError(f"cannot take a pointer of {type(x)}")
 
 
+def _addr(x):
+    """`_ptr` as a plain number, which ctypes passes as it is: a decode step's calls have a dozen of them and take 10 us."""
+    try:
+        return x.data_ptr()
+    except AttributeError:
+        return None if x is None else _ptr(x).value
+
+
 def _host(a, name, shape=None):
     if not isinstance(a, np.ndarray) or a.dtype != np.float32 or not a.flags["C_CONTIGUOUS"]:
         raise TypeError(f"{name} must be a C-contiguous float32 numpy array")
@@ -33,12 +41,17 @@ def _host(a, name, shape=None):
 
 
 _DTYPES = {"float32": N.F32, "bfloat16": N.BF16, "float16": N.F16}
+_TORCH_DTYPES = {}  # the same by a tensor's dtype, as they are met
 
 
 def _dtype(x, given, name):
     """The element type of a device buffer: of the tensor, or the one named ("float32", "bfloat16", "float16") for a raw pointer."""
     own = getattr(x, "dtype", None)
+    if given is None and own in _TORCH_DTYPES:
+        return _TORCH_DTYPES[own]
     key = str(own).removeprefix("torch.") if own is not None else given
+    if key in _DTYPES and own is not None and given is None:
+        _TORCH_DTYPES[own] = _DTYPES[key]
     if key not in _DTYPES or (given is not None and given != key):
         raise TypeError(f"{name} must be float32, bfloat16 or float16 (name the type of a raw pointer): got {key}" +
                         (f", {given} asked for" if own is not None and given is not None else ""))
@@ -286,8 +299,8 @@ class B200Dispatch:
         [rows, 2] is what the gradient call takes back. `dtype` names the logits' type where they are a raw pointer. See
         pssa_b200_token_logprobs_dev in include/pssa_b200.h for masked rows and rows without a target."""
         self._check(self._lib.pssa_b200_token_logprobs_dev(
-            self._h, _ptr(logits), _dtype(logits, dtype, "logits"), rows, vocab, vocab if ld is None else ld, temperature, _ptr(targets),
-            _ptr(logprob), _ptr(rank), _ptr(entropy), _ptr(stats), top_n, _ptr(top_ids), _ptr(top_logprobs)))
+            self._h, _addr(logits), _dtype(logits, dtype, "logits"), rows, vocab, vocab if ld is None else ld, temperature, _addr(targets),
+            _addr(logprob), _addr(rank), _addr(entropy), _addr(stats), top_n, _addr(top_ids), _addr(top_logprobs)))
 
     def token_logprobs_grad_dev(self, logits, rows, vocab, targets, stats, grad_logits, grad_logprob=None, entropy=None,
                                 grad_entropy=None, temperature=1.0, ld=None, ld_grad=None, dtype=None):
@@ -296,8 +309,8 @@ class B200Dispatch:
         if _dtype(grad_logits, dtype, "grad_logits") != _dtype(logits, dtype, "logits"):
             raise TypeError("grad_logits must have the type of the logits")
         self._check(self._lib.pssa_b200_token_logprobs_grad_dev(
-            self._h, _ptr(logits), _dtype(logits, dtype, "logits"), rows, vocab, vocab if ld is None else ld, temperature, _ptr(targets),
-            _ptr(stats), _ptr(entropy), _ptr(grad_logprob), _ptr(grad_entropy), _ptr(grad_logits), vocab if ld_grad is None else ld_grad))
+            self._h, _addr(logits), _dtype(logits, dtype, "logits"), rows, vocab, vocab if ld is None else ld, temperature, _addr(targets),
+            _addr(stats), _addr(entropy), _addr(grad_logprob), _addr(grad_entropy), _addr(grad_logits), vocab if ld_grad is None else ld_grad))
 
     def distill_topk_dev(self, logits, rows, vocab, teacher_ids, teacher, k, kl=None, grad_kl=None, targets=None, ce=None, grad_ce=None,
                          grad_logits=None, temperature=1.0, teacher_temperature=1.0, rest=False, ld=None, ld_grad=None, dtype=None):
@@ -307,15 +320,15 @@ class B200Dispatch:
         if grad_logits is not None and _dtype(grad_logits, dtype, "grad_logits") != _dtype(logits, dtype, "logits"):
             raise TypeError("grad_logits must have the type of the logits")
         self._check(self._lib.pssa_b200_distill_topk_dev(
-            self._h, _ptr(logits), _dtype(logits, dtype, "logits"), rows, vocab, vocab if ld is None else ld, temperature,
-            _ptr(teacher_ids), _ptr(teacher), k, teacher_temperature, _ptr(targets), N.DISTILL_REST if rest else 0, _ptr(kl), _ptr(ce),
-            _ptr(grad_kl), _ptr(grad_ce), _ptr(grad_logits), vocab if ld_grad is None else ld_grad))
+            self._h, _addr(logits), _dtype(logits, dtype, "logits"), rows, vocab, vocab if ld is None else ld, temperature,
+            _addr(teacher_ids), _addr(teacher), k, teacher_temperature, _addr(targets), N.DISTILL_REST if rest else 0, _addr(kl), _addr(ce),
+            _addr(grad_kl), _addr(grad_ce), _addr(grad_logits), vocab if ld_grad is None else ld_grad))
 
     # ---- products with 4-bit weights (device pointers)
     def w4_quantize_dev(self, w, n, k, group, codes, scales, zeros=None, dtype=None, scale_dtype=None):
         """The matrix w [n, k] as 4-bit codes [n, k/2] with a scale (and, with `zeros`, a zero) for each `group` of columns."""
-        self._check(self._lib.pssa_b200_w4_quantize_dev(self._h, _ptr(w), _dtype(w, dtype, "w"), n, k, group, _ptr(codes), _ptr(scales),
-                                                        _dtype(scales, scale_dtype, "scales"), _ptr(zeros)))
+        self._check(self._lib.pssa_b200_w4_quantize_dev(self._h, _addr(w), _dtype(w, dtype, "w"), n, k, group, _addr(codes), _addr(scales),
+                                                        _dtype(scales, scale_dtype, "scales"), _addr(zeros)))
 
     def gemv_w4_dev(self, x, rows, codes, scales, zeros, n, k, group, out, ldx=None, ldo=None, epilogue=N.EPI_NONE, alpha=1.0,
                     dtype=None, scale_dtype=None):
@@ -323,8 +336,8 @@ class B200Dispatch:
         if _dtype(out, dtype, "out") != _dtype(x, dtype, "x"):
             raise TypeError("out must have the type of x")
         self._check(self._lib.pssa_b200_gemv_w4_dev(
-            self._h, _ptr(x), _dtype(x, dtype, "x"), rows, k if ldx is None else ldx, _ptr(codes), _ptr(scales),
-            _dtype(scales, scale_dtype, "scales"), _ptr(zeros), n, k, group, _ptr(out), n if ldo is None else ldo, epilogue, alpha))
+            self._h, _addr(x), _dtype(x, dtype, "x"), rows, k if ldx is None else ldx, _addr(codes), _addr(scales),
+            _dtype(scales, scale_dtype, "scales"), _addr(zeros), n, k, group, _addr(out), n if ldo is None else ldo, epilogue, alpha))
 
     # ---- bank write / plastic fast weights (device pointers)
     def bank_insert_protected_dev(self, keys, norm_sq, values, confidence, last_seen_step, meta, capacity, d_key, d_val,
