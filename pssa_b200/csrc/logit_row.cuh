@@ -123,11 +123,11 @@ __device__ __forceinline__ float vector_max(uint4 v, const float (&x)[kVec<T>]) 
 // every vector, and following each cost 1.5 times the pass (4096 x 131072 bf16: 237 us, now 168). Sums stay below 2^4 a logit and lose nothing. It is never below the
 // lowest finite number: a row of that value alone is a distribution like any other, a row of -inf is none. A difference is formed before it is
 // scaled, so that logits far from zero lose nothing. A NaN or +inf makes `sum` a NaN, or `top` infinite.
-template <bool ENTROPY>
+template <bool ENTROPY, bool WHERE = false>
 struct SoftmaxSums {
     float top = -INFINITY, ref = -FLT_MAX, lim = -FLT_MAX;
     F2 sum = {0}, ent = {0};  // sum 2^t, sum 2^t t with t = (x - ref) c; 64 bits of 0 are a pair of zeros
-    int where = -1;           // the first vector that holds `top`
+    int where = -1;           // WHERE: the first vector that holds `top`
 
     __device__ __forceinline__ void start(float m, float c) {
         if (m > ref) ref = m, lim = m + 4.0f / c;
@@ -142,7 +142,7 @@ struct SoftmaxSums {
     // N elements whose largest is m
     template <int N>
     __device__ __forceinline__ void add(const float (&x)[N], float m, int at, float c) {
-        where = m > top ? at : where;
+        if (WHERE) where = m > top ? at : where;
         top = fmaxf(top, m);
         if (m > lim) raise(m, c);
         const F2 nref = pair(-ref, -ref), c2 = pair(c, c);

@@ -22,6 +22,7 @@ namespace cg = cooperative_groups;
 using Key = unsigned long long;
 
 constexpr int kRoom = 1024;  // candidates of a CTA
+constexpr int kMaxCtas = 8;  // of a cluster
 
 struct RowPart {  // a CTA's numbers for its cluster
     float top, ref, sum, ent;
@@ -30,7 +31,7 @@ struct RowPart {  // a CTA's numbers for its cluster
 
 template <int THREADS>
 struct LogprobShared {
-    RowPart part;
+    RowPart part, parts[kMaxCtas];
     float f[3][THREADS / 32];
     unsigned u[THREADS / 32];
     Key bound, wide[THREADS / 32];
@@ -154,7 +155,7 @@ __device__ void best_of_part(const Part<T>& part, Key own, int n, LogprobShared<
 }
 
 template <typename T, int THREADS, bool TOP>
-__global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LogprobParams p, int ctas) {
+__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 5 : 1) token_logprobs_kernel(LogprobParams p, int ctas) {
     __shared__ LogprobShared<THREADS> s;
     constexpr int kWarps = THREADS / 32, N = kVec<T>, kAhead = 4;
     const size_t row = blockIdx.x / (unsigned)ctas;
@@ -167,7 +168,7 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LogprobParams p
     const bool has = t < (uint32_t)v, none = t == PSSA_B200_NO_TOKEN;
     const float xt = has ? to_f32(x[t]) : INFINITY;
 
-    SoftmaxSums<true> sums;
+    SoftmaxSums<true, TOP> sums;
     unsigned above = 0;
     auto take = [&](uint4 raw, int at) {
         float f[N];
@@ -250,14 +251,20 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LogprobParams p
     if (TOP) best_of_part<T, THREADS>(part, own, p.top_n, s);
     // the cluster's
     const cg::cluster_group cluster = cg::this_cluster();
-    if (ctas > 1)
+    if (ctas > 1) {
         cluster.sync();
-    else
-        __syncthreads();
+        if (rank == 0) {  // everything at once into this CTA's memory: one trip, not one for every step of the search below
+            if (tid < ctas) s.parts[tid] = *cluster.map_shared_rank(&s.part, tid);
+            if (TOP)
+                for (int i = tid; i < p.top_n * ctas; i += THREADS) s.found[i] = cluster.map_shared_rank(s.best, i / p.top_n)[i % p.top_n];
+        }
+        cluster.barrier_arrive();
+    }
+    __syncthreads();
     if (rank == 0) {
-        RowPart all = s.part;
+        RowPart all = ctas > 1 ? s.parts[0] : s.part;
         for (int i = 1; i < ctas; ++i) {
-            RowPart o = *cluster.map_shared_rank(&s.part, i);
+            RowPart o = s.parts[i];
             const float to = fmaxf(all.ref, o.ref);
             rebase(all.ref, to, c, all.sum, all.ent);
             rebase(o.ref, to, c, o.sum, o.ent);
@@ -285,12 +292,12 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LogprobParams p
             } else {  // a key's place is the number of better ones: its own list is in order, the others are searched
                 for (int i = tid; i < n * ctas; i += THREADS) {
                     const int list = i / n, at_ = i - list * n;
-                    const Key k = cluster.map_shared_rank(s.best, list)[at_];
+                    const Key k = s.found[i];
                     if (k == 0) continue;
                     int place = at_;
                     for (int l = 0; l < ctas; ++l) {
                         if (l == list) continue;
-                        const Key* o = cluster.map_shared_rank(s.best, l);
+                        const Key* o = s.found + l * n;
                         int lo = 0, hi = n;  // the first that is not better
                         while (lo < hi) {
                             const int mid = (lo + hi) >> 1;
@@ -307,7 +314,7 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LogprobParams p
             }
         }
     }
-    if (ctas > 1) cluster.sync();  // no CTA leaves while its numbers are read
+    if (ctas > 1) cluster.barrier_wait();  // no CTA leaves while its numbers are read
 }
 
 // d = p (A + B lp) + (at the target) g, lp = log2 p: one read, one write. A CTA takes `span` vectors of one row; rows that start at different
@@ -384,8 +391,8 @@ cudaError_t launch_rows(pssa_b200_ctx* ctx, const LogprobParams& p, int ctas) {
 
 int32_t launch_token_logprobs(pssa_b200_ctx* ctx, const LogprobParams& p) {
     const size_t vecs = (size_t)p.vocab * dtype_size(p.dtype) / 16;
-    int ctas = 1;  // of a row: until the GPU has two of them to an SM, or a thread would have no vector left
-    while (ctas < 8 && p.rows * ctas < (size_t)ctx->sm_count * 2 && vecs / (ctas * 2) >= 256) ctas *= 2;
+    int ctas = 1;  // of a row: until the GPU has one to an SM, or a thread would have no vector left. A cluster costs 3 us (256 rows of 16384 with 5 alternatives: 8.1 us, 11.0 as pairs)
+    while (ctas < kMaxCtas && p.rows * ctas < (size_t)ctx->sm_count && vecs / (ctas * 2) >= 256) ctas *= 2;
     const bool few = p.rows * ctas <= (size_t)ctx->sm_count && vecs / ctas >= 2048;  // more threads, where few CTAs have long parts
     if (p.rows * ctas > 0x7fffffffull) return fail(ctx, PSSA_B200_ERR_SHAPE, "B200 log probabilities: too many rows; refusing launch");
     const cudaError_t e = with_dtype(p.dtype, [&](auto t) {
