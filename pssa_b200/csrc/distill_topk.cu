@@ -144,7 +144,7 @@ struct RestSums {  // of a CTA's unlisted ids: sums at the temperature, and at 1
     float top, ref, sum, sum1;
 };
 struct Teacher {  // what one warp makes of a row's entries while the row is on its way
-    uint32_t id[PSSA_B200_MAX_TEACHER];  // PSSA_B200_NO_TOKEN: absent
+    alignas(16) uint32_t id[PSSA_B200_MAX_TEACHER];  // PSSA_B200_NO_TOKEN: absent, and behind the last up to a multiple of 4
     float t[PSSA_B200_MAX_TEACHER], log_t[PSSA_B200_MAX_TEACHER], x[PSSA_B200_MAX_TEACHER];
     float t_at[PSSA_B200_MAX_TEACHER];   // the id's whole mass at its first entry, -1 at others of it
     float x_max, rest, mass;             // of the listed logits; 1 - sum t, with DISTILL_REST; sum t + rest
@@ -153,7 +153,7 @@ struct Teacher {  // what one warp makes of a row's entries while the row is on 
 
 // run by one warp; k entries in steps of 32
 template <typename T>
-__device__ void read_teacher(const DistillParams& p, size_t row, const T* x, uint32_t tgt, Teacher& s, bool report) {
+__device__ void read_teacher(const DistillParams& p, size_t row, const T* x, Teacher& s, bool report) {
     const int lane = threadIdx.x & 31, v = p.vocab;
     const float inv = 1.0f / p.teacher_temperature;
     float q_max = -INFINITY, x_max = -INFINITY;
@@ -170,12 +170,8 @@ __device__ void read_teacher(const DistillParams& p, size_t row, const T* x, uin
     if (report && wrong) atomicExch(p.status, PSSA_B200_ERR_TOKEN);
     float rest = 0.0f, mass = 0.0f;
     if (p.rest) {
-        double sum = 0.0;
-        for (int i = lane; i < p.k; i += 32) {
-            const float q = s.log_t[i];
-            s.t[i] = expf(q);
-            sum += exp((double)q);
-        }
+        double sum = 0.0;  // of fp32 numbers: their difference from 1 is what is left
+        for (int i = lane; i < p.k; i += 32) sum += s.t[i] = expf(s.log_t[i]);
 #pragma unroll
         for (int m = 16; m > 0; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
         if (__any_sync(0xffffffffu, any)) rest = fmaxf((float)(1.0 - sum), 0.0f);  // no entry: nothing to learn
@@ -191,21 +187,9 @@ __device__ void read_teacher(const DistillParams& p, size_t row, const T* x, uin
         for (int i = lane; i < p.k; i += 32) s.t[i] = sum != 0.0f ? s.t[i] / sum : 0.0f, s.log_t[i] = s.log_t[i] - q_max - log_sum;
     }
     for (int i = lane; i < p.k; i += 32) mass += s.t[i];
-    __syncwarp();
-    int target = -1;
-    for (int i = lane; i < p.k; i += 32) {
-        const uint32_t id = s.id[i];
-        float t_at = 0.0f;
-        bool first = id != PSSA_B200_NO_TOKEN;
-        if (first)
-            for (int j = 0; j < p.k; ++j)
-                if (s.id[j] == id) first = first && j >= i, t_at += s.t[j];
-        s.t_at[i] = first ? t_at : -1.0f;
-        if (first && id == tgt) target = i;
-    }
-    x_max = warp_max(x_max), mass = warp_sum(mass) + rest;
-    target = __reduce_max_sync(0xffffffffu, target), bad = __any_sync(0xffffffffu, bad);
-    if (lane == 0) s.x_max = x_max, s.rest = rest, s.mass = mass, s.bad = bad, s.target = target;
+    if (lane < 3 && p.k + lane < PSSA_B200_MAX_TEACHER) s.id[p.k + lane] = PSSA_B200_NO_TOKEN;
+    x_max = warp_max(x_max), mass = warp_sum(mass) + rest, bad = __any_sync(0xffffffffu, bad);
+    if (lane == 0) s.x_max = x_max, s.rest = rest, s.mass = mass, s.bad = bad, s.target = -1;
 }
 
 // A CTA holds elements [rank * each, + each) of a row, at the distance from a 16-byte boundary that they have in global memory.
@@ -243,7 +227,7 @@ __global__ void __launch_bounds__(kThreads) distill_topk_kernel(DistillParams p,
     const float inv_t = 1.0f / p.temperature, c = kLog2e / p.temperature;
     const uint32_t tgt = p.targets ? p.targets[row] : PSSA_B200_NO_TOKEN;
     const bool has = tgt < (uint32_t)v, none = tgt == PSSA_B200_NO_TOKEN;
-    if (warp == 0) read_teacher(p, row, x, has ? tgt : PSSA_B200_NO_TOKEN - 1, s_teacher, rank == 0);
+    if (warp == 0) read_teacher(p, row, x, s_teacher, rank == 0);
     const float w_kl = p.grad_kl ? p.grad_kl[row] : 0.0f, w_ce = p.grad_ce && has ? p.grad_ce[row] : 0.0f;
     float xt = -INFINITY;
     if (tid == 0 && rank == 0) {
@@ -251,11 +235,25 @@ __global__ void __launch_bounds__(kThreads) distill_topk_kernel(DistillParams p,
         if (!has && !none) atomicExch(p.status, PSSA_B200_ERR_TOKEN);
     }
     __syncthreads();  // the entries, and the barrier
+    // a thread to an entry: is it the first of its id, and what is the id's whole mass? (k = 64: one warp took as long as the row's way here)
+    const uint32_t id = tid < p.k ? s_teacher.id[tid] : PSSA_B200_NO_TOKEN;
+    if (tid < p.k) {
+        bool first = id != PSSA_B200_NO_TOKEN;
+        float t_at = 0.0f;
+        for (int j = 0; j < p.k; j += 4) {
+            const uint4 o = *reinterpret_cast<const uint4*>(s_teacher.id + j);
+            if (o.x == id) first = first && j >= tid, t_at += s_teacher.t[j];
+            if (o.y == id) first = first && j + 1 >= tid, t_at += s_teacher.t[j + 1];
+            if (o.z == id) first = first && j + 2 >= tid, t_at += s_teacher.t[j + 2];
+            if (o.w == id) first = first && j + 3 >= tid, t_at += s_teacher.t[j + 3];
+        }
+        s_teacher.t_at[tid] = first ? t_at : -1.0f;
+        if (first && id == tgt) s_teacher.target = tid;
+    }
     if (vecs && !tc::mbar_wait(&s_bar, 0)) {
         atomicExch(p.status, PSSA_B200_ERR_TIMEOUT);
         tc::mbar_wait(&s_bar, 0);  // no CTA leaves with its copy on the way, if a wait can help it
     }
-    const uint32_t id = tid < p.k ? s_teacher.id[tid] : PSSA_B200_NO_TOKEN;
     const bool mine = id >= (uint32_t)e0 && id < (uint32_t)e1;
     if (mine) held[id - e0] = from_f32<T>(-INFINITY);
     __syncthreads();
