@@ -140,6 +140,7 @@ __global__ void __launch_bounds__(kThreads) distill_topk_long_kernel(DistillPara
     }
 }
 
+constexpr int kPartThreads = 256, kPartWarps = kPartThreads / 32;
 struct RestSums {  // of a CTA's unlisted ids: sums at the temperature, and at 1
     float top, ref, sum, sum1;
 };
@@ -194,10 +195,10 @@ __device__ void read_teacher(const DistillParams& p, size_t row, const T* x, Tea
 
 // A CTA holds elements [rank * each, + each) of a row, at the distance from a 16-byte boundary that they have in global memory.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) distill_topk_kernel(DistillParams p, int ctas, int each) {
+__global__ void __launch_bounds__(kPartThreads) distill_topk_kernel(DistillParams p, int ctas, int each) {
     extern __shared__ __align__(128) unsigned char s_raw[];
     __shared__ Teacher s_teacher;
-    __shared__ float s_top[kWarps], s_ref[kWarps], s_sum[kWarps], s_sum1[kWarps];
+    __shared__ float s_top[kPartWarps], s_ref[kPartWarps], s_sum[kPartWarps], s_sum1[kPartWarps];
     __shared__ RestSums s_part;
     __shared__ __align__(8) uint64_t s_bar;
     constexpr int N = kVec<T>;
@@ -271,7 +272,8 @@ __global__ void __launch_bounds__(kThreads) distill_topk_kernel(DistillParams p,
         rest.start(m, c), rest1.start(m, kLog2e);
     }
     auto sweep = [&](auto both) {
-        for (int i = tid; i < vecs; i += kThreads) {
+#pragma unroll 2
+        for (int i = tid; i < vecs; i += kPartThreads) {
             const uint4 raw = held_vec[i];
             float f[N];
             unpack<T>(raw, f);
@@ -301,25 +303,32 @@ __global__ void __launch_bounds__(kThreads) distill_topk_kernel(DistillParams p,
         if (lane == 0) s_top[warp] = top, s_ref[warp] = ref, s_sum[warp] = sum, s_sum1[warp] = two ? sum1 : sum;
     }
     __syncthreads();
-    auto join = [&](RestSums& a, RestSums b) {
-        const float to = fmaxf(a.ref, b.ref);
-        float unused = 0.0f;
-        rebase(a.ref, to, c, a.sum, unused);
-        rebase(b.ref, to, c, b.sum, unused);
-        if (two) {
-            rebase(a.ref, to, kLog2e, a.sum1, unused);
-            rebase(b.ref, to, kLog2e, b.sum1, unused);
+    // eight parts, one to a lane of each eight; every thread gets the same sums
+    auto join = [&](RestSums a) {
+        float to = a.ref, unused = 0.0f;
+#pragma unroll
+        for (int i = 4; i > 0; i >>= 1) {
+            to = fmaxf(to, __shfl_xor_sync(0xffffffffu, to, i));
+            a.top = fmaxf(a.top, __shfl_xor_sync(0xffffffffu, a.top, i));
         }
-        a.ref = to, a.top = fmaxf(a.top, b.top), a.sum += b.sum, a.sum1 += b.sum1;
+        rebase(a.ref, to, c, a.sum, unused);
+        if (two) rebase(a.ref, to, kLog2e, a.sum1, unused);
+        a.ref = to;
+#pragma unroll
+        for (int i = 4; i > 0; i >>= 1) {
+            a.sum += __shfl_xor_sync(0xffffffffu, a.sum, i);
+            if (two) a.sum1 += __shfl_xor_sync(0xffffffffu, a.sum1, i);
+        }
+        return a;
     };
-    RestSums all{s_top[0], s_ref[0], s_sum[0], s_sum1[0]};
-    for (int i = 1; i < kWarps; ++i) join(all, RestSums{s_top[i], s_ref[i], s_sum[i], s_sum1[i]});
+    static_assert(kPartWarps == 8, "a part to a lane of eight");
+    const int eighth = lane & 7;
+    RestSums all = join(RestSums{s_top[eighth], s_ref[eighth], s_sum[eighth], s_sum1[eighth]});
     const cg::cluster_group cluster = cg::this_cluster();
     if (ctas > 1) {
         if (tid == 0) s_part = all;
         cluster.sync();  // and every CTA has read the listed logits: from here on their places may be written
-        all = *cluster.map_shared_rank(&s_part, 0);
-        for (int i = 1; i < ctas; ++i) join(all, *cluster.map_shared_rank(&s_part, i));
+        all = join(eighth < ctas ? *cluster.map_shared_rank(&s_part, eighth) : RestSums{-INFINITY, -FLT_MAX, 0.0f, 0.0f});
         cluster.barrier_arrive();
     }
     // with the listed ids: everything relative to the row's maximum m, the rest's sum to its own
@@ -358,28 +367,40 @@ __global__ void __launch_bounds__(kThreads) distill_topk_kernel(DistillParams p,
         const float nref = -all.ref;
         T* out = static_cast<T*>(p.grad) + row * p.ld_grad + e0;
         const bool together = ((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(from)) & 15) == 0;
-        auto write = [&](auto grad) {
+        auto write = [&](auto grad) {  // of a pair of logits
+            auto grad1 = [&](T v) {
+                float y, unused;
+                split(grad(pair(to_f32(v), 0.0f)), y, unused);
+                return from_f32<T>(y);
+            };
             if (together) {
                 uint4* out_vec = reinterpret_cast<uint4*>(out + head);
-                for (int i = tid; i < vecs; i += kThreads) {
+#pragma unroll 2
+                for (int i = tid; i < vecs; i += kPartThreads) {
                     float f[N];
                     unpack<T>(held_vec[i], f);
 #pragma unroll
-                    for (int e = 0; e < N; ++e) f[e] = grad(f[e]);
+                    for (int e = 0; e < N; e += 2) split(grad(pair(f[e], f[e + 1])), f[e], f[e + 1]);
                     out_vec[i] = pack<T>(f);
                 }
-                if (tid < head) out[tid] = from_f32<T>(grad(to_f32(held[tid])));
-                if (tail0 + tid < n) out[tail0 + tid] = from_f32<T>(grad(to_f32(held[tail0 + tid])));
+                if (tid < head) out[tid] = grad1(held[tid]);
+                if (tail0 + tid < n) out[tail0 + tid] = grad1(held[tail0 + tid]);
             } else {
-                for (int i = tid; i < n; i += kThreads) out[i] = from_f32<T>(grad(to_f32(held[i])));
+                for (int i = tid; i < n; i += kPartThreads) out[i] = grad1(held[i]);
             }
         };
+        auto powers = [&](F2 t) {
+            float x0, x1;
+            split(t, x0, x1);
+            return pair(ex2(x0), ex2(x1));
+        };
+        const F2 nref2 = pair(nref, nref), c2 = pair(c, c), log2e2 = pair(kLog2e, kLog2e), both2 = pair(both, both), a12 = pair(a1, a1);
         if (zero || bad) {
             const float y = zero ? 0.0f : kNan;
-            write([&](float) { return y; });
+            write([&](F2) { return pair(y, y); });
         } else {
-            auto one = [&](float f) { return both * ex2((f + nref) * c); };
-            auto with_ce = [&](float f) { return fmaf(a1, ex2((f + nref) * kLog2e), both * ex2((f + nref) * c)); };
+            auto one = [&](F2 f) { return mul2(both2, powers(mul2(add2(f, nref2), c2))); };
+            auto with_ce = [&](F2 f) { return fma2(a12, powers(mul2(add2(f, nref2), log2e2)), one(f)); };
             const bool ce2 = two && w_ce != 0.0f;
             if (ce2)
                 write(with_ce);
@@ -393,8 +414,11 @@ __global__ void __launch_bounds__(kThreads) distill_topk_kernel(DistillParams p,
                 if (w_ce != 0.0f) d += w_ce * (expf(xe - m) / s1 - (id == tgt ? 1.0f : 0.0f));
                 out[id - e0] = from_f32<T>(d);
             }
-            if (tid == 0 && w_ce != 0.0f && s_teacher.target < 0 && tgt >= (uint32_t)e0 && tgt < (uint32_t)e1)
-                out[tgt - e0] = from_f32<T>((ce2 ? with_ce(xt_here) : one(xt_here)) - w_ce);
+            if (tid == 0 && w_ce != 0.0f && s_teacher.target < 0 && tgt >= (uint32_t)e0 && tgt < (uint32_t)e1) {
+                float y, unused;
+                split(ce2 ? with_ce(pair(xt_here, 0.0f)) : one(pair(xt_here, 0.0f)), y, unused);
+                out[tgt - e0] = from_f32<T>(y - w_ce);
+            }
         }
     }
     if (ctas > 1) cluster.barrier_wait();  // no CTA leaves while its sums are read
@@ -410,7 +434,7 @@ int32_t launch_parts(pssa_b200_ctx* ctx, const DistillParams& p, int ctas) {
         attr.done(ctx->device);
     }
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(p.rows * ctas)), cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = smem, cfg.stream = ctx->stream;
+    cfg.gridDim = dim3((unsigned)(p.rows * ctas)), cfg.blockDim = dim3(kPartThreads), cfg.dynamicSmemBytes = smem, cfg.stream = ctx->stream;
     cudaLaunchAttribute at{};
     at.id = cudaLaunchAttributeClusterDimension;
     at.val.clusterDim.x = ctas, at.val.clusterDim.y = 1, at.val.clusterDim.z = 1;
