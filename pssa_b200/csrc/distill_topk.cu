@@ -140,11 +140,12 @@ __global__ void __launch_bounds__(kThreads) distill_topk_long_kernel(DistillPara
     }
 }
 
-constexpr int kPartThreads = 256, kPartWarps = kPartThreads / 32;
+// eight warps read the row and one the teacher's entries; the row comes in pieces, each with a barrier of its own
+constexpr int kRowWarps = 8, kPartThreads = 32 * (kRowWarps + 1), kPieces = 4;
 struct RestSums {  // of a CTA's unlisted ids: sums at the temperature, and at 1
     float top, ref, sum, sum1;
 };
-struct Teacher {  // what one warp makes of a row's entries while the row is on its way
+struct Teacher {  // what one warp makes of a row's entries while the others read the row
     alignas(16) uint32_t id[PSSA_B200_MAX_TEACHER];  // PSSA_B200_NO_TOKEN: absent, and behind the last up to a multiple of 4
     float t[PSSA_B200_MAX_TEACHER], log_t[PSSA_B200_MAX_TEACHER], x[PSSA_B200_MAX_TEACHER];
     float t_at[PSSA_B200_MAX_TEACHER];   // the id's whole mass at its first entry, -1 at others of it
@@ -152,9 +153,12 @@ struct Teacher {  // what one warp makes of a row's entries while the row is on 
     int bad, target;                     // a listed logit is no number; the target's entry or -1
 };
 
-// run by one warp; k entries in steps of 32
+// where the warp of the teacher and those of the row meet
+__device__ __forceinline__ void ids_ready() { asm volatile("bar.sync 1, %0;" ::"n"(kPartThreads) : "memory"); }
+
+// Run by one warp, the entries in steps of 32, behind its barrier with the others, who need the ids.
 template <typename T>
-__device__ void read_teacher(const DistillParams& p, size_t row, const T* x, Teacher& s, bool report) {
+__device__ void read_teacher(const DistillParams& p, size_t row, const T* x, uint32_t tgt, Teacher& s, bool report) {
     const int lane = threadIdx.x & 31, v = p.vocab;
     const float inv = 1.0f / p.teacher_temperature;
     float q_max = -INFINITY, x_max = -INFINITY;
@@ -162,13 +166,20 @@ __device__ void read_teacher(const DistillParams& p, size_t row, const T* x, Tea
     for (int i = lane; i < p.k; i += 32) {
         const uint32_t id = p.teacher_ids[row * p.k + i];
         const bool entry = id < (uint32_t)v;
+        wrong |= !entry && id != PSSA_B200_NO_TOKEN, any |= entry;
+        s.id[i] = entry ? id : PSSA_B200_NO_TOKEN;
+    }
+    if (lane < 3 && p.k + lane < PSSA_B200_MAX_TEACHER) s.id[p.k + lane] = PSSA_B200_NO_TOKEN;
+    ids_ready();
+    if (report && wrong) atomicExch(p.status, PSSA_B200_ERR_TOKEN);
+    for (int i = lane; i < p.k; i += 32) {
+        const uint32_t id = s.id[i];
+        const bool entry = id != PSSA_B200_NO_TOKEN;
         const float q = entry ? p.teacher[row * p.k + i] * inv : -INFINITY, xe = entry ? to_f32(x[id]) : -INFINITY;
-        wrong |= !entry && id != PSSA_B200_NO_TOKEN;
-        any |= entry, bad |= xe != xe;
-        s.id[i] = entry ? id : PSSA_B200_NO_TOKEN, s.x[i] = xe, s.log_t[i] = q;
+        bad |= xe != xe;
+        s.x[i] = xe, s.log_t[i] = q;
         q_max = fmaxf(q_max, q != q ? INFINITY : q), x_max = fmaxf(x_max, xe);
     }
-    if (report && wrong) atomicExch(p.status, PSSA_B200_ERR_TOKEN);
     float rest = 0.0f, mass = 0.0f;
     if (p.rest) {
         double sum = 0.0;  // of fp32 numbers: their difference from 1 is what is left
@@ -188,9 +199,25 @@ __device__ void read_teacher(const DistillParams& p, size_t row, const T* x, Tea
         for (int i = lane; i < p.k; i += 32) s.t[i] = sum != 0.0f ? s.t[i] / sum : 0.0f, s.log_t[i] = s.log_t[i] - q_max - log_sum;
     }
     for (int i = lane; i < p.k; i += 32) mass += s.t[i];
-    if (lane < 3 && p.k + lane < PSSA_B200_MAX_TEACHER) s.id[p.k + lane] = PSSA_B200_NO_TOKEN;
-    x_max = warp_max(x_max), mass = warp_sum(mass) + rest, bad = __any_sync(0xffffffffu, bad);
-    if (lane == 0) s.x_max = x_max, s.rest = rest, s.mass = mass, s.bad = bad, s.target = -1;
+    __syncwarp();
+    // is an entry the first of its id, and what is the id's whole mass?
+    int target = -1;
+    for (int i = lane; i < p.k; i += 32) {
+        const uint32_t id = s.id[i];
+        bool first = id != PSSA_B200_NO_TOKEN;
+        float t_at = 0.0f;
+        for (int j = 0; j < p.k; j += 4) {
+            const uint4 o = *reinterpret_cast<const uint4*>(s.id + j);
+            if (o.x == id) first = first && j >= i, t_at += s.t[j];
+            if (o.y == id) first = first && j + 1 >= i, t_at += s.t[j + 1];
+            if (o.z == id) first = first && j + 2 >= i, t_at += s.t[j + 2];
+            if (o.w == id) first = first && j + 3 >= i, t_at += s.t[j + 3];
+        }
+        s.t_at[i] = first ? t_at : -1.0f;
+        if (first && id == tgt) target = i;
+    }
+    x_max = warp_max(x_max), mass = warp_sum(mass) + rest, bad = __any_sync(0xffffffffu, bad), target = __reduce_max_sync(0xffffffffu, target);
+    if (lane == 0) s.x_max = x_max, s.rest = rest, s.mass = mass, s.bad = bad, s.target = target;
 }
 
 // A CTA holds elements [rank * each, + each) of a row, at the distance from a 16-byte boundary that they have in global memory.
@@ -198,9 +225,9 @@ template <typename T>
 __global__ void __launch_bounds__(kPartThreads) distill_topk_kernel(DistillParams p, int ctas, int each) {
     extern __shared__ __align__(128) unsigned char s_raw[];
     __shared__ Teacher s_teacher;
-    __shared__ float s_top[kPartWarps], s_ref[kPartWarps], s_sum[kPartWarps], s_sum1[kPartWarps];
+    __shared__ float s_top[kRowWarps], s_ref[kRowWarps], s_sum[kRowWarps], s_sum1[kRowWarps];
     __shared__ RestSums s_part;
-    __shared__ __align__(8) uint64_t s_bar;
+    __shared__ __align__(8) uint64_t s_bar[kPieces];
     constexpr int N = kVec<T>;
     const size_t row = blockIdx.x / (unsigned)ctas;
     const int rank = blockIdx.x % (unsigned)ctas, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, v = p.vocab;
@@ -213,13 +240,15 @@ __global__ void __launch_bounds__(kPartThreads) distill_topk_kernel(DistillParam
     const int vecs = (n - head) / N, tail0 = head + vecs * N;
     T* held = reinterpret_cast<T*>(s_raw) + off;
     uint4* held_vec = reinterpret_cast<uint4*>(held + head);
+    const int piece = (vecs + kPieces - 1) / kPieces;
     if (tid == 0) {
-        tc::mbar_init(&s_bar, 1);
+        for (int i = 0; i < kPieces; ++i) tc::mbar_init(&s_bar[i], 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        if (vecs) {
-            tc::mbar_expect_tx(&s_bar, vecs * 16);
-            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(tc::smem_u32(held_vec)),
-                         "l"(from + head), "r"(vecs * 16), "r"(tc::smem_u32(&s_bar))
+        for (int i = 0; i * piece < vecs; ++i) {
+            const int bytes = (min((i + 1) * piece, vecs) - i * piece) * 16;
+            tc::mbar_expect_tx(&s_bar[i], bytes);
+            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(tc::smem_u32(held_vec + i * piece)),
+                         "l"(from + head + (size_t)i * piece * N), "r"(bytes), "r"(tc::smem_u32(&s_bar[i]))
                          : "memory");
         }
     }
@@ -228,72 +257,69 @@ __global__ void __launch_bounds__(kPartThreads) distill_topk_kernel(DistillParam
     const float inv_t = 1.0f / p.temperature, c = kLog2e / p.temperature;
     const uint32_t tgt = p.targets ? p.targets[row] : PSSA_B200_NO_TOKEN;
     const bool has = tgt < (uint32_t)v, none = tgt == PSSA_B200_NO_TOKEN;
-    if (warp == 0) read_teacher(p, row, x, s_teacher, rank == 0);
     const float w_kl = p.grad_kl ? p.grad_kl[row] : 0.0f, w_ce = p.grad_ce && has ? p.grad_ce[row] : 0.0f;
     float xt = -INFINITY;
     if (tid == 0 && rank == 0) {
         if (has) xt = to_f32(x[tgt]);
         if (!has && !none) atomicExch(p.status, PSSA_B200_ERR_TOKEN);
     }
-    __syncthreads();  // the entries, and the barrier
-    // a thread to an entry: is it the first of its id, and what is the id's whole mass? (k = 64: one warp took as long as the row's way here)
-    const uint32_t id = tid < p.k ? s_teacher.id[tid] : PSSA_B200_NO_TOKEN;
-    if (tid < p.k) {
-        bool first = id != PSSA_B200_NO_TOKEN;
-        float t_at = 0.0f;
-        for (int j = 0; j < p.k; j += 4) {
-            const uint4 o = *reinterpret_cast<const uint4*>(s_teacher.id + j);
-            if (o.x == id) first = first && j >= tid, t_at += s_teacher.t[j];
-            if (o.y == id) first = first && j + 1 >= tid, t_at += s_teacher.t[j + 1];
-            if (o.z == id) first = first && j + 2 >= tid, t_at += s_teacher.t[j + 2];
-            if (o.w == id) first = first && j + 3 >= tid, t_at += s_teacher.t[j + 3];
-        }
-        s_teacher.t_at[tid] = first ? t_at : -1.0f;
-        if (first && id == tgt) s_teacher.target = tid;
-    }
-    if (vecs && !tc::mbar_wait(&s_bar, 0)) {
-        atomicExch(p.status, PSSA_B200_ERR_TIMEOUT);
-        tc::mbar_wait(&s_bar, 0);  // no CTA leaves with its copy on the way, if a wait can help it
-    }
-    const bool mine = id >= (uint32_t)e0 && id < (uint32_t)e1;
-    if (mine) held[id - e0] = from_f32<T>(-INFINITY);
-    __syncthreads();
-
-    // the sums of the ids that are not listed; at temperature 1 they serve the cross entropy too
     const bool two = p.targets && p.temperature != 1.0f;
-    SoftmaxSums<false> rest, rest1;
-    {
-        float f[N], m = -INFINITY;
-        if (tid < vecs) {
-            unpack<T>(held_vec[tid], f);
-            m = vector_max<T>(held_vec[tid], f);
-        }
-        m = warp_max(m);
-        rest.start(m, c), rest1.start(m, kLog2e);
-    }
-    auto sweep = [&](auto both) {
+    if (warp == kRowWarps) {
+        read_teacher(p, row, x, has ? tgt : PSSA_B200_NO_TOKEN - 1, s_teacher, rank == 0);
+    } else {
+        ids_ready();  // and the barriers
+        // the sums of the ids that are not listed; at temperature 1 they serve the cross entropy too. Each warp masks the listed ids of its own share.
+        SoftmaxSums<false> rest, rest1;
+        auto mask = [&](auto mine) {
+            for (int i = lane; i < p.k; i += 32) {
+                const uint32_t id = s_teacher.id[i];
+                if (id >= (uint32_t)e0 && id < (uint32_t)e1 && mine((int)id - e0)) held[(int)id - e0] = from_f32<T>(-INFINITY);
+            }
+            __syncwarp();
+        };
+        auto sweep = [&](int lo, int hi, auto both) {
 #pragma unroll 2
-        for (int i = tid; i < vecs; i += kPartThreads) {
-            const uint4 raw = held_vec[i];
-            float f[N];
-            unpack<T>(raw, f);
-            const float m = vector_max<T>(raw, f);
-            rest.add(f, m, 0, c);
-            if (both) rest1.add(f, m, 0, kLog2e);
+            for (int i = lo + lane; i < hi; i += 32) {
+                const uint4 raw = held_vec[i];
+                float f[N];
+                unpack<T>(raw, f);
+                const float m = vector_max<T>(raw, f);
+                rest.add(f, m, 0, c);
+                if (both) rest1.add(f, m, 0, kLog2e);
+            }
+        };
+        for (int i = 0; i * piece < vecs; ++i) {
+            if (!tc::mbar_wait(&s_bar[i], 0)) {
+                if (lane == 0) atomicExch(p.status, PSSA_B200_ERR_TIMEOUT);
+                tc::mbar_wait(&s_bar[i], 0);  // no CTA leaves with its copy on the way, if a wait can help it
+            }
+            const int last = min((i + 1) * piece, vecs), share = (last - i * piece + kRowWarps - 1) / kRowWarps;
+            const int lo = min(i * piece + warp * share, last), hi = min(lo + share, last);
+            mask([&](int at) { return at >= head + lo * N && at < head + hi * N; });
+            if (i == 0) {
+                float f[N], m = -INFINITY;
+                if (lo + lane < hi) {
+                    unpack<T>(held_vec[lo + lane], f);
+                    m = vector_max<T>(held_vec[lo + lane], f);
+                }
+                m = warp_max(m);
+                rest.start(m, c), rest1.start(m, kLog2e);
+            }
+            if (two)
+                sweep(lo, hi, std::true_type());
+            else
+                sweep(lo, hi, std::false_type());
         }
-    };
-    if (two)
-        sweep(std::true_type());
-    else
-        sweep(std::false_type());
-    auto single = [&](int i) {
-        const float f = to_f32(held[i]);
-        rest.add1(f, c);
-        if (two) rest1.add1(f, kLog2e);
-    };
-    if (tid < head) single(tid);
-    if (tail0 + tid < n) single(tail0 + tid);
-    {
+        if (warp == 0) {
+            mask([&](int at) { return at < head || at >= tail0; });
+            auto single = [&](int i) {
+                const float f = to_f32(held[i]);
+                rest.add1(f, c);
+                if (two) rest1.add1(f, kLog2e);
+            };
+            if (tid < head) single(tid);
+            if (tail0 + tid < n) single(tail0 + tid);
+        }
         const float ref = warp_max(fmaxf(rest.ref, rest1.ref)), top = warp_max(rest.top);
         float sum = rest.total(), sum1 = rest1.total(), unused = 0.0f;
         rebase(rest.ref, ref, c, sum, unused);
@@ -321,7 +347,7 @@ __global__ void __launch_bounds__(kPartThreads) distill_topk_kernel(DistillParam
         }
         return a;
     };
-    static_assert(kPartWarps == 8, "a part to a lane of eight");
+    static_assert(kRowWarps == 8, "a part to a lane of eight");
     const int eighth = lane & 7;
     RestSums all = join(RestSums{s_top[eighth], s_ref[eighth], s_sum[eighth], s_sum1[eighth]});
     const cg::cluster_group cluster = cg::this_cluster();
@@ -406,6 +432,8 @@ __global__ void __launch_bounds__(kPartThreads) distill_topk_kernel(DistillParam
                 write(with_ce);
             else
                 write(one);
+            const uint32_t id = tid < p.k ? s_teacher.id[tid] : PSSA_B200_NO_TOKEN;
+            const bool mine = id >= (uint32_t)e0 && id < (uint32_t)e1;
             const float xt_here = has && tgt >= (uint32_t)e0 && tgt < (uint32_t)e1 ? to_f32(held[tgt - e0]) : 0.0f;
             __syncthreads();  // the listed ids and the target go over what has been written
             if (mine && s_teacher.t_at[tid] >= 0.0f) {
