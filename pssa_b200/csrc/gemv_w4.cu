@@ -403,7 +403,7 @@ __device__ __forceinline__ void store_scale(void* scales, int dtype, size_t i, f
 struct GroupForm {
     float step, inv;
     int zero;
-    bool live;
+    bool live, exact;  // exact: 1 / step is no normal number, or quotients are too large for the short way (a scale cut to its type's largest number)
 };
 template <int LANES>
 __device__ __forceinline__ GroupForm group_form(const W4Params& p, size_t at, float lo, float hi, bool bad, bool store) {
@@ -423,6 +423,7 @@ __device__ __forceinline__ GroupForm group_form(const W4Params& p, size_t at, fl
     f.step = step, f.live = step > 0.0f;
     f.zero = !p.zeros ? 8 : f.live ? (int)fminf(fmaxf(rintf(__fdiv_rn(-lo, step)), 0.0f), 15.0f) : 0;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(f.inv) : "f"(step));
+    f.exact = !(f.inv >= FLT_MIN && f.inv <= FLT_MAX && fmaxf(hi, -lo) * f.inv < 64.0f);
     if (store && p.zeros) p.zeros[at] = (uint8_t)f.zero;
     return f;
 }
@@ -436,11 +437,11 @@ __device__ __noinline__ unsigned exact_code(float a, float step, int zero) {
 __device__ __forceinline__ unsigned codes_of(const GroupForm& f, const float* x) {
     if (!f.live) return 0x11111111u * (unsigned)f.zero;
     constexpr float kRound = 12582912.0f;
-    float middle = f.inv >= FLT_MIN && f.inv <= FLT_MAX ? 0.0f : 1.0f;
+    float middle = f.exact ? 1.0f : 0.0f;
     unsigned word = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        const float v = fminf(fmaxf(x[j] * f.inv, -32.0f), 32.0f), r = v + kRound;
+        const float v = x[j] * f.inv, r = v + kRound;
         middle = fmaxf(middle, fabsf(v - (r - kRound)));
         const int q = __float_as_int(r) - (__float_as_int(kRound) - f.zero);
         word |= (unsigned)min(max(q, 0), 15) << 4 * j;
@@ -458,47 +459,59 @@ __device__ __forceinline__ unsigned codes_of(const GroupForm& f, const float* x)
     return word;
 }
 
-// Groups of LANES * 16 columns, 32 / LANES of them to a warp at a time and AHEAD times that on their way: one read of the weights. A lane's 16 codes are
-// 8 bytes. w starts on 16 bytes. 16384 x 8192 bf16 with zeros: 167 us with 8 columns a lane and a conversion a weight.
+// Groups of LANES * 32 columns, 32 / LANES of them to a warp: one read of the weights, in units of 8 columns that neighbouring lanes hold in turn. What a group
+// costs besides its weights, two divisions first of all, is shared by 32 of them (16384 x 8192 bf16 with zeros: 141 us with 16 to a lane, 167 with 8). w starts on 16 bytes.
 template <typename T, int LANES>
 __global__ void __launch_bounds__(kThreads) w4_quantize_groups_kernel(W4Params p, const T* __restrict__ w) {
-    constexpr int kWords = sizeof(T), kAhead = sizeof(T) == 4 ? 1 : 2;  // 16-byte words of 16 columns
-    const size_t total = p.n * p.groups, step = kThreads / LANES, at0 = (size_t)blockIdx.x * step * kAhead + threadIdx.x / LANES;
+    constexpr int kUnits = 4, kWords = sizeof(T) / 2;  // units of a lane; 16-byte words of a unit
+    const size_t total = p.n * p.groups, at = ((size_t)blockIdx.x * kThreads + threadIdx.x) / LANES;
     const int lane = threadIdx.x % LANES;
-    uint4 raw[kAhead][kWords];
-    size_t off[kAhead];
-    bool in[kAhead];
+    const size_t n = total >> 32 ? at / p.groups : (unsigned)at / (unsigned)p.groups, k0 = (at - n * p.groups) * p.group, row = n * p.k;
+    const int left = at < total ? (int)min(p.group, p.k - k0) : 0;  // columns of the group
+    uint4 raw[kUnits][kWords];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-        const size_t at = at0 + i * step, n = total >> 32 ? at / p.groups : (unsigned)at / (unsigned)p.groups, k = (at - n * p.groups) * p.group + 16 * lane;
-        in[i] = at < total && k < p.k, off[i] = n * p.k + k;
+    for (int u = 0; u < kUnits; ++u) {
+        const int k = (u * LANES + lane) * 8;
 #pragma unroll
-        for (int j = 0; j < kWords; ++j) raw[i][j] = in[i] ? reinterpret_cast<const uint4*>(w + off[i])[j] : make_uint4(0, 0, 0, 0);
+        for (int j = 0; j < kWords; ++j) raw[u][j] = k < left ? reinterpret_cast<const uint4*>(w + row + k0 + k)[j] : make_uint4(0, 0, 0, 0);
     }
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-        float x[16], lo = 0.0f, hi = 0.0f;
-        bool bad = false;
-#pragma unroll
-        for (int j = 0; j < kWords; ++j) unpack<T>(raw[i][j], *reinterpret_cast<float(*)[kVec<T>]>(x + j * kVec<T>));
+    auto unit = [&](int u, float (&x)[8]) {
         if constexpr (sizeof(T) == 4) {
-            float none = 0.0f;  // a NaN once a weight is none or infinite
-#pragma unroll
-            for (int j = 0; j < 16; ++j) lo = fminf(lo, x[j]), hi = fmaxf(hi, x[j]), none = fmaf(x[j], 0.0f, none);
-            bad = none != none;
-        } else {  // two at a time, as they lie; a NaN stays one
-            using T2 = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
-            const T2* h = reinterpret_cast<const T2*>(raw[i]);
-            T2 a = h[0], b = h[0];
-#pragma unroll
-            for (int j = 1; j < 8; ++j) a = __hmin2_nan(a, h[j]), b = __hmax2_nan(b, h[j]);
-            lo = fminf(to_f32(a.x), to_f32(a.y)), hi = fmaxf(to_f32(b.x), to_f32(b.y));
-            const float none = fmaf(to_f32(a.x), 0.0f, fmaf(to_f32(a.y), 0.0f, fmaf(to_f32(b.x), 0.0f, to_f32(b.y) * 0.0f)));
-            bad = none != none, lo = fminf(lo, 0.0f), hi = fmaxf(hi, 0.0f);
+            unpack<T>(raw[u][0], *reinterpret_cast<float(*)[4]>(x));
+            unpack<T>(raw[u][1], *reinterpret_cast<float(*)[4]>(x + 4));
+        } else {
+            unpack<T>(raw[u][0], x);
         }
-        const size_t at = at0 + i * step;
-        const GroupForm f = group_form<LANES>(p, at, lo, hi, bad, lane == 0 && at < total);
-        if (in[i]) *reinterpret_cast<uint2*>(p.codes + (off[i] >> 1)) = make_uint2(codes_of(f, x), codes_of(f, x + 8));
+    };
+    float lo = 0.0f, hi = 0.0f;
+    bool bad = false;
+    if constexpr (sizeof(T) == 4) {
+        float none = 0.0f;  // a NaN once a weight is none or infinite
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u) {
+            float x[8];
+            unit(u, x);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) lo = fminf(lo, x[j]), hi = fmaxf(hi, x[j]), none = fmaf(x[j], 0.0f, none);
+        }
+        bad = none != none;
+    } else {  // two at a time, as they lie; a NaN stays one
+        using T2 = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+        const T2* h = reinterpret_cast<const T2*>(raw);
+        T2 a = h[0], b = h[0];
+#pragma unroll
+        for (int j = 1; j < kUnits * 4; ++j) a = __hmin2_nan(a, h[j]), b = __hmax2_nan(b, h[j]);
+        lo = fminf(to_f32(a.x), to_f32(a.y)), hi = fmaxf(to_f32(b.x), to_f32(b.y));
+        const float none = fmaf(to_f32(a.x), 0.0f, fmaf(to_f32(a.y), 0.0f, fmaf(to_f32(b.x), 0.0f, to_f32(b.y) * 0.0f)));
+        bad = none != none, lo = fminf(lo, 0.0f), hi = fmaxf(hi, 0.0f);
+    }
+    const GroupForm f = group_form<LANES>(p, at, lo, hi, bad, lane == 0 && left > 0);
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+        const int k = (u * LANES + lane) * 8;
+        float x[8];
+        unit(u, x);
+        if (k < left) *reinterpret_cast<unsigned*>(p.codes + (row + k0 + k >> 1)) = codes_of(f, x);
     }
 }
 
@@ -529,7 +542,7 @@ __global__ void __launch_bounds__(kThreads) w4_quantize_kernel(W4Params p, const
 int32_t launch_w4_quantize(pssa_b200_ctx* ctx, const W4Params& w, const void* src, int dtype) {
     // lanes of a group share a warp evenly
     const bool together = w.group <= 512 && (w.group & (w.group - 1)) == 0 && (reinterpret_cast<uintptr_t>(src) & 15) == 0;
-    const size_t lanes = together ? w.group / 16 : 32, per = kThreads / lanes * (together && dtype != PSSA_B200_F32 ? 2 : 1), blocks = (w.n * w.groups + per - 1) / per;
+    const size_t lanes = together ? w.group / 32 : 32, per = kThreads / lanes, blocks = (w.n * w.groups + per - 1) / per;
     if (blocks > 0x7fffffff) return fail(ctx, PSSA_B200_ERR_SHAPE, "B200 4-bit weights: too many groups; refusing launch");
     with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
@@ -537,16 +550,16 @@ int32_t launch_w4_quantize(pssa_b200_ctx* ctx, const W4Params& w, const void* sr
         const unsigned grid = (unsigned)blocks;
         if (!together)
             w4_quantize_kernel<<<grid, kThreads, 0, ctx->stream>>>(w, x);
+        else if (lanes == 1)
+            w4_quantize_groups_kernel<T, 1><<<grid, kThreads, 0, ctx->stream>>>(w, x);
         else if (lanes == 2)
             w4_quantize_groups_kernel<T, 2><<<grid, kThreads, 0, ctx->stream>>>(w, x);
         else if (lanes == 4)
             w4_quantize_groups_kernel<T, 4><<<grid, kThreads, 0, ctx->stream>>>(w, x);
         else if (lanes == 8)
             w4_quantize_groups_kernel<T, 8><<<grid, kThreads, 0, ctx->stream>>>(w, x);
-        else if (lanes == 16)
-            w4_quantize_groups_kernel<T, 16><<<grid, kThreads, 0, ctx->stream>>>(w, x);
         else
-            w4_quantize_groups_kernel<T, 32><<<grid, kThreads, 0, ctx->stream>>>(w, x);
+            w4_quantize_groups_kernel<T, 16><<<grid, kThreads, 0, ctx->stream>>>(w, x);
     });
     return after_launch(ctx, together ? "w4_quantize_groups_kernel" : "w4_quantize_kernel");
 }
