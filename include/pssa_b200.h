@@ -373,26 +373,27 @@ typedef enum pssa_b200_dtype {
 
 /*
  * A weight matrix [n, k] in 4 bits (no counterpart in the reference, whose weights are fp32): codes [n, k/2] bytes, the even
- * column in a byte's low half; scales [n, G] of type `scale_dtype` and, when given, zeros [n, G] bytes in 0..15, one of each for
- * every `group` consecutive columns of a row, G = ceil(k / group) (a last group may be shorter). The weight of a code c is
+ * column in a byte's low half; scales [n, G] of type `scale_dtype` and, when given, zeros [n, G] bytes in 0..15, one of each
+ * for every `group` consecutive columns of a row, G = ceil(k / group) (a last group may be shorter). The weight of a code c is
  * (c - zero) * scale; without zeros, zero is 8. k is a multiple of 32; group is 32, 64 or a multiple of 128 (at most k rounded
  * up to 128). Rows and groups are dense; codes start on a 16-byte boundary, scales on their type's.
  *
  * pssa_b200_w4_quantize_dev makes that form of w [n, k] (`dtype`, dense) by rounding to nearest even. Without zeros: scale =
- * max|w| / 7 and c = clamp(rint(w / scale), -8, 7) + 8. With zeros: lo = min(w, 0), hi = max(w, 0) over the group, scale =
- * (hi - lo) / 15, zero = clamp(rint(-lo / scale), 0, 15), c = clamp(rint(w / scale) + zero, 0, 15). Scales are rounded to their
+ * max|w| / 7 and c = clamp(rint(w / scale), -8, 7) + 8. With zeros: lo = min(w, 0), hi = max(w, 0) over the group, scale = (hi
+ * - lo) / 15, zero = clamp(rint(-lo / scale), 0, 15), c = clamp(rint(w / scale) + zero, 0, 15). Scales are rounded to their
  * type (to its largest finite value where they are above it) before they are used. A group whose scale is 0 gets codes that
- * stand for 0; a group with a NaN or an infinity gets a NaN scale, and products with it are NaN.
+ * stand for 0; a group with a NaN or an infinity gets a NaN scale, and products with it are NaN. The arrays must not overlap.
  */
 int32_t pssa_b200_w4_quantize_dev(pssa_b200_ctx* ctx, const void* w, int32_t dtype, size_t n, size_t k, size_t group, uint8_t* codes,
                                   void* scales, int32_t scale_dtype, uint8_t* zeros);
 /*
  * Y[rows, n] = epilogue(X[rows, k] * W[n, k]^T) with W in 4 bits, for the few rows of a decode step: pssa_b200_gemm_xwt_dev's
- * contract (epilogues and alpha included) with the weights read at a quarter of a bf16 matrix's bytes. x (row pitch ldx >= k) and
- * out (row pitch ldo >= n) are of type `dtype`, element-aligned; sums are fp32, one rounding to `dtype` at the end. Code times
- * input is exact for bf16 and fp16 inputs and, for fp32, good to 2^-22 of the input (it goes through three bf16 pieces, of
- * which the smallest is dropped below the normal range); the scale is applied to each group's fp32 sum. A row's bits
- * do not depend on the number of rows. x and out must not overlap. Only enqueues; needs no workspace.
+ * contract (epilogues and alpha included) with the weights read at a quarter of a bf16 matrix's bytes. x (row pitch ldx >= k)
+ * and out (row pitch ldo >= n) are of type `dtype`, element-aligned; sums are fp32, one rounding to `dtype` at the end. Code
+ * times input is exact: an fp32 input goes through as three bf16 pieces of its bits, as far down as bf16 reaches (2^-133). The
+ * scale is applied to the fp32 sum of each group, or of each 128 columns of a longer one. A NaN among a row's inputs makes its
+ * results NaN, an infinity makes them NaN or infinite, and no other row's. A row's bits do not depend on the other rows, but
+ * may on their number. k is at most 8388480. out must not overlap the other arrays. Only enqueues; needs no workspace.
  */
 int32_t pssa_b200_gemv_w4_dev(pssa_b200_ctx* ctx, const void* x, int32_t dtype, size_t rows, size_t ldx, const uint8_t* codes,
                               const void* scales, int32_t scale_dtype, const uint8_t* zeros, size_t n, size_t k, size_t group, void* out,
@@ -541,19 +542,19 @@ int32_t pssa_b200_sample_dev(pssa_b200_ctx* ctx, float* logits, float* probs, si
 #define PSSA_B200_MAX_TEACHER 256
 
 /*
- * Log probabilities of given tokens, with rank, entropy and the best alternatives, of `rows` rows of logits (`dtype`, row pitch
- * ld >= vocab elements, element-aligned) at a temperature T > 0. The reference scores a target's cross entropy only
+ * Log probabilities of given tokens, with rank, entropy and the best alternatives, of `rows` rows of logits (`dtype`, row
+ * pitch ld >= vocab elements, element-aligned) at a temperature T > 0. The reference scores a target's cross entropy only
  * (src/pssa.rs:2597-2750) and reports the sampled id's probability (`raw_confidence`, src/inference.rs:526-545).
  *   z_v = (x_v - max x) / T,  l = ln sum exp z,  logprob = z_target - l,  rank = 1 + #{v: x_v > x_target},
  *   entropy = l - sum p_v z_v (nats),  stats = {max x, l}: what the gradient call takes back,
  *   top_ids / top_logprobs [rows, top_n]: the top_n largest by (logit desc, id asc) in that order; PSSA_B200_NO_TOKEN and -inf
  *   behind the last id when top_n > vocab.
- * All DEVICE pointers: targets [rows] u32 (NULL when neither logprob nor rank is wanted; PSSA_B200_NO_TOKEN: logprob 0, rank 0;
- * another id outside the vocabulary: logprob NaN, rank 0, and PSSA_B200_ERR_TOKEN in the context's status word), logprob, entropy
- * [rows], stats [rows, 2], rank [rows] u32; each output may be NULL. top_n <= PSSA_B200_MAX_TOP.
- * Logits of -inf are masked ids: probability 0, log probability -inf. A row of nothing else has logprob -inf, entropy 0, stats
- * {-inf, 0}, rank 1. A row that holds a NaN or +inf has no distribution: its fp32 results are NaN, rank 0, top_ids
- * PSSA_B200_NO_TOKEN. A row's bits do not depend on the other rows, but may on their number.
+ * All DEVICE pointers: targets [rows] u32 (NULL when neither logprob nor rank is wanted; PSSA_B200_NO_TOKEN: logprob 0, rank
+ * 0; another id outside the vocabulary: logprob NaN, rank 0, and PSSA_B200_ERR_TOKEN in the context's status word), logprob,
+ * entropy [rows], stats [rows, 2], rank [rows] u32; each output may be NULL. top_n <= PSSA_B200_MAX_TOP. Logits of -inf are
+ * masked ids: probability 0, log probability -inf. A row of nothing else has logprob -inf, entropy 0, stats {-inf, 0}, rank 1.
+ * A row that holds a NaN or +inf has no distribution: its fp32 results are NaN, rank 0, top_ids PSSA_B200_NO_TOKEN. A row's
+ * bits do not depend on the other rows, but may on their number.
  */
 int32_t pssa_b200_token_logprobs_dev(pssa_b200_ctx* ctx, const void* logits, int32_t dtype, size_t rows, size_t vocab, size_t ld,
                                      float temperature, const uint32_t* targets, float* logprob, uint32_t* rank, float* entropy,
@@ -563,9 +564,10 @@ int32_t pssa_b200_token_logprobs_dev(pssa_b200_ctx* ctx, const void* logits, int
  *   grad_logits_v = (1 / T) (grad_logprob (1[v = target] - p_v) - grad_entropy p_v (ln p_v + entropy)),
  * with stats [rows, 2] and entropy [rows] as the forward call gave them for the same logits and T. grad_logprob / grad_entropy
  * [rows]: either may be NULL (zero); grad_logprob needs targets, grad_entropy needs entropy. grad_logits (`dtype`, row pitch
- * ld_grad >= vocab) may be the logits themselves with the same pitch (in place), and must not overlap them otherwise. A row whose
- * weights are both zero, or that has no token and no entropy weight, gets a zero gradient whatever its logits hold, and so does a
- * row of masked ids only. Other ids outside the vocabulary count as no token and raise PSSA_B200_ERR_TOKEN in the status word.
+ * ld_grad >= vocab) may be the logits themselves with the same pitch (in place), and must not overlap them otherwise. A row
+ * whose weights are both zero, or that has no token and no entropy weight, gets a zero gradient whatever its logits hold, and
+ * so does a row of masked ids only; a row without a distribution gets NaN. Other ids outside the vocabulary count as no token
+ * and raise PSSA_B200_ERR_TOKEN in the status word.
  */
 int32_t pssa_b200_token_logprobs_grad_dev(pssa_b200_ctx* ctx, const void* logits, int32_t dtype, size_t rows, size_t vocab, size_t ld,
                                           float temperature, const uint32_t* targets, const float* stats, const float* entropy,
@@ -575,8 +577,8 @@ int32_t pssa_b200_token_logprobs_grad_dev(pssa_b200_ctx* ctx, const void* logits
  * listed. Without it the teacher is the softmax of its entries. */
 #define PSSA_B200_DISTILL_REST 1u
 /*
- * Distillation from a teacher's best ids (no counterpart in the reference): per row the divergence of the student from the teacher
- * and, in the same call, the gradient with respect to the student's logits. With p = softmax(x / temperature):
+ * Distillation from a teacher's best ids (no counterpart in the reference): per row the divergence of the student from the
+ * teacher and, in the same call, the gradient with respect to the student's logits. With p = softmax(x / temperature):
  *   t = softmax(teacher / teacher_temperature) over the row's entries,  kl = sum t_i (ln t_i - ln p[id_i]);
  *   with PSSA_B200_DISTILL_REST (teacher_temperature must be 1): t_i = exp(teacher_i), r = max(1 - sum t_i, 0), p_rest = the
  *   sum of p over the ids that are not listed, kl = sum t_i (ln t_i - ln p[id_i]) + r (ln r - ln p_rest);
@@ -585,12 +587,13 @@ int32_t pssa_b200_token_logprobs_grad_dev(pssa_b200_ctx* ctx, const void* logits
  * All DEVICE pointers: logits / grad_logits (`dtype`, pitches ld, ld_grad >= vocab; grad_logits may be NULL, or the logits
  * themselves with the same pitch), teacher_ids u32 and teacher fp32 [rows, k] (k <= PSSA_B200_MAX_TEACHER; what
  * pssa_b200_token_logprobs_dev gives as top_ids and top_logprobs fits), kl, ce [rows] (NULL to skip), grad_kl, grad_ce [rows]
- * (needed with grad_logits for the losses that are to be trained; NULL: zero), targets [rows] (needed by ce and grad_ce).
- * An id of PSSA_B200_NO_TOKEN is an absent entry or target: it counts nothing, and a row without entries has kl 0. An id that is
- * listed twice has the sum of its entries' mass. Other ids outside the vocabulary raise PSSA_B200_ERR_TOKEN in the status word
- * and count as absent (ce NaN). ln p is held in fp32 and is -inf below its range. Masked student logits (-inf) under a teacher's mass give kl = +inf and a finite gradient; a row of masked ids only
- * gives kl (where the teacher has mass) and ce +inf and a zero gradient. A row with a NaN or +inf gives NaN. A row whose gradient weights are all zero
- * gets a zero gradient whatever its logits hold.
+ * (needed with grad_logits for the losses that are to be trained; NULL: zero), targets [rows] (needed by ce and grad_ce). An
+ * id of PSSA_B200_NO_TOKEN is an absent entry or target: it counts nothing, and a row without entries has kl 0. An id that is
+ * listed twice has the sum of its entries' mass. vocab is at most 1638400. Other ids outside the vocabulary raise
+ * PSSA_B200_ERR_TOKEN in the status word and count as absent (ce NaN). ln p is held in fp32 and is -inf below its range.
+ * Masked student logits (-inf) under a teacher's mass give kl = +inf and a finite gradient; a row of masked ids only gives kl
+ * (where the teacher has mass) and ce +inf and a zero gradient. A row with a NaN or +inf gives NaN. A row whose gradient
+ * weights are all zero gets a zero gradient whatever its logits hold.
  */
 int32_t pssa_b200_distill_topk_dev(pssa_b200_ctx* ctx, const void* logits, int32_t dtype, size_t rows, size_t vocab, size_t ld,
                                    float temperature, const uint32_t* teacher_ids, const float* teacher, size_t k,

@@ -1,5 +1,4 @@
 // Products of a few rows with a matrix in 4 bits, and quantisation to that form (see pssa_b200_gemv_w4_dev).
-// One warp to a weight row, or to a group that is quantised.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -17,15 +16,23 @@ constexpr int kThreads = 256;
 
 // ---- product
 //
-// out[r, n] = sum over groups of scale * sum over the group's columns of (code - zero) * x. Code minus zero is a small whole number, exact in
-// bf16 and fp16, so the inner sums go through mma.m16n8k16 with 16 weight rows as A, the inputs' rows as the 8 columns of B and fp32
-// accumulators, and only a group's sum meets the scale. An fp32 input is three columns, its bits cut into three bf16 numbers that add up to it.
+// out[r, n] = sum over groups of scale * sum over the group's columns of (code - zero) * x. Code minus zero is a small whole
+// number, exact in bf16 and fp16, so the inner sums go through mma.m16n8k16 with 16 weight rows as A, the inputs' rows as the 8
+// columns of B and fp32 accumulators, and only a group's sum meets the scale. An fp32 input is three columns, its bits cut into
+// three bf16 numbers that add up to it.
 //
-// A chunk is 128 columns. Lane (g, t) of a warp (g = lane / 4, t = lane % 4) loads 16 bytes, 32 codes, of rows g and g + 8, so that a row's chunk
-// is 64 bytes in a row. Which columns the four lanes of a row multiply at a time is free as long as A and B agree, but all of one product have
-// to be of one group: as they lie for groups of 128 and more, after one exchange between lanes two apart for 64, after a 4 x 4
-// transposition for 32. `run_placed` says which run of 8 columns is where. A word's 8 codes become 4 registers of two columns 4 apart, by a mask and the bits
-// of 128 (fp16: 1024) that put a code into a mantissa; x is staged with its runs in that order.
+// A chunk is 128 columns. Lane (g, t) of a warp (g = lane / 4, t = lane % 4) loads 16 bytes, 32 codes, of rows g and g + 8, so that
+// a row's chunk is 64 bytes in a row. Which columns the four lanes of a row multiply at a time is free as long as A and B agree,
+// but all of one product have to be of one group: as they lie for groups of 128 and more, after one exchange between lanes two
+// apart for 64, after a 4 x 4 transposition for 32. `run_placed` says which run of 8 columns is where. A word's 8 codes become 4
+// registers of two columns 4 apart, by a mask and the bits of 128 (fp16: 1024) that put a code into a mantissa; x is staged with
+// its runs in that order.
+//
+// What bounds it: one row of 32768 x 8192 takes 40 us, 3.4 TB/s, of which 38 stay when all loads hit the same chunk: the 11
+// instructions that make 8 codes into numbers, at 16 warps an SM. 48 rows of 16384 x 4096 take 43 us: staging 11, joining and
+// storing 11, products and conversions the rest, one after another since every SM has one or two CTAs in step. Codes through a
+// ring of bulk copies (73 us: a barrier and a trip for the scales per piece) and one tile of rows a warp with three chunks on
+// their way (58 us: the work per chunk beside the conversion, twice as often) were slower.
 constexpr int kWarps = kThreads / 32;
 constexpr int kChunk = 128;
 
@@ -177,8 +184,9 @@ constexpr int ctas_per_sm(int nt) { return nt <= 2 ? 2 : 1; }
 constexpr int kMaxCols = 48;  // of B at a time
 
 // MODE 0: groups of 128 and more, 1: of 64, 2: of 32.
-// A CTA: kWarps / k_warps warps side by side over weight rows, each with MT times 16 of them, times k_warps over the columns' chunks; NT times 8 columns of B. A warp has the
-// codes of its next chunk on their way while it multiplies one. The CTAs of a cluster split the columns further; the first of them joins their sums. Sums are joined in a fixed order.
+// A CTA: kWarps / k_warps warps side by side over weight rows, each with MT times 16 of them, times k_warps over the columns'
+// chunks; NT times 8 columns of B. A warp has the codes of its next chunk on their way while it multiplies one. The CTAs of a
+// cluster split the columns further and each joins the sums of a part of the rows. Sums are joined in a fixed order.
 template <typename T, int NT, int MT, int MODE>
 __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) gemv_w4_kernel(GemvW4Params p, W4Split sp) {
     extern __shared__ uint4 s_x[];
@@ -193,8 +201,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) gemv_w4_kernel(Gemv
     const size_t row_bytes = p.w.k >> 1;
     const int k = (int)p.w.k;
 
-    // This lane's weight rows are g + 8 m of the warp's; those behind the last row are not fetched, multiply what was there before and are not stored. It fetches the scales
-    // and zeros of the t-th of them, for its quad. Inputs behind the last column are staged as 0: any codes serve there.
+    // This lane's weight rows are g + 8 m of the warp's; those behind the last row are not fetched, multiply what was there before
+    // and are not stored. It fetches the scales and zeros of the t-th of them, for its quad. Inputs behind the last column are
+    // staged as 0: any codes serve there.
     const size_t n_lane = n0 + (size_t)wm * MT * 16 + g;
     const int left = n_lane < p.w.n ? (int)min(p.w.n - n_lane, (size_t)MT * 16) : 0;
     const uint8_t* codes = p.w.codes + (left ? n_lane : 0) * row_bytes;
@@ -234,7 +243,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) gemv_w4_kernel(Gemv
     for (int j = 0; j < NT; ++j) col_at[j] = min(j * 8 + g, cols - 1) * 4 + t;
 
     const T* x = static_cast<const T*>(p.x) + r0 * p.ldx;
-    // 16 threads to a chunk's runs of one row; the others take other rows, or chunks where there are few rows. Lanes next to each other store to different banks.
+    // 16 threads to a chunk's runs of one row; the others take other rows, or chunks where there are few rows. Lanes next to each
+    // other store to different banks.
     const int run_at = threadIdx.x & 3, run_word = threadIdx.x >> 3 & 3, lot = (threadIdx.x >> 5) * 2 + (threadIdx.x >> 2 & 1);
     const int run = run_placed<MODE>(run_word, run_at), row_lots = 1 << sp.row_lots_log, chunk_lots = kThreads / 16 >> sp.row_lots_log;
     auto stage = [&](int first) {
@@ -403,7 +413,7 @@ __device__ __forceinline__ void store_scale(void* scales, int dtype, size_t i, f
 struct GroupForm {
     float step, inv;
     int zero;
-    bool live, exact;  // exact: 1 / step is no normal number, or quotients are too large for the short way (a scale cut to its type's largest number)
+    bool live, exact;  // exact: 1 / step is no normal number, or quotients are too large for the short way (a scale cut to its type)
 };
 template <int LANES>
 __device__ __forceinline__ GroupForm group_form(const W4Params& p, size_t at, float lo, float hi, bool bad, bool store) {
@@ -431,9 +441,10 @@ __device__ __forceinline__ GroupForm group_form(const W4Params& p, size_t at, fl
 __device__ __noinline__ unsigned exact_code(float a, float step, int zero) {
     return (unsigned)fminf(fmaxf(rintf(__fdiv_rn(a, step)) + (float)zero, 0.0f), 15.0f);
 }
-// The same for 8 weights, as one word. The product with 1 / step is within 3e-6 of the quotient where that is below 16, so that both round to the same whole
-// number unless it lies within 1e-5 of the middle of two; there, and where 1 / step is no number, the division decides, out of line. Adding 1.5 * 2^23 rounds to a
-// whole number and leaves it in the low bits: a conversion for each weight would be bound by the units that convert.
+// The same for 8 weights, as one word. The product with 1 / step is within 3e-6 of the quotient where that is below 16, so that
+// both round to the same whole number unless it lies within 1e-5 of the middle of two; there, and where 1 / step is no normal
+// number, the division decides, out of line. Adding 1.5 * 2^23 rounds to a whole number and leaves it in the low bits: a
+// conversion for each weight would be bound by the units that convert (167 us for 16384 x 8192 bf16, now 129).
 __device__ __forceinline__ unsigned codes_of(const GroupForm& f, const float* x) {
     if (!f.live) return 0x11111111u * (unsigned)f.zero;
     constexpr float kRound = 12582912.0f;
@@ -459,8 +470,9 @@ __device__ __forceinline__ unsigned codes_of(const GroupForm& f, const float* x)
     return word;
 }
 
-// Groups of LANES * 32 columns, 32 / LANES of them to a warp: one read of the weights, in units of 8 columns that neighbouring lanes hold in turn. What a group
-// costs besides its weights, two divisions first of all, is shared by 32 of them (16384 x 8192 bf16 with zeros: 141 us with 16 to a lane, 167 with 8). w starts on 16 bytes.
+// Groups of LANES * 32 columns, 32 / LANES of them to a warp: one read of the weights, in units of 8 columns that neighbouring
+// lanes hold in turn. What a group costs besides its weights, two divisions first of all, is shared by 32 of them (16384 x 8192
+// bf16 with zeros: 129 us, 2.6 TB/s; 141 with 16 to a lane). Bound by the instructions of the codes. w starts on 16 bytes.
 template <typename T, int LANES>
 __global__ void __launch_bounds__(kThreads) w4_quantize_groups_kernel(W4Params p, const T* __restrict__ w) {
     constexpr int kUnits = 4, kWords = sizeof(T) / 2;  // units of a lane; 16-byte words of a unit
@@ -577,8 +589,9 @@ int32_t launch_tiles(pssa_b200_ctx* ctx, const GemvW4Params& p, int slice) {
     sp.vec = (reinterpret_cast<uintptr_t>(p.x) & 15) == 0 && p.ldx * sizeof(T) % 16 == 0;
     sp.slice = slice;
     while (1 << sp.row_lots_log < slice && sp.row_lots_log < 4) ++sp.row_lots_log;
-    // Warps take columns rather than rows while the GPU has room for the CTAs, two to an SM (head of 16384 x 768, 1 row: 6.8, 6.2, 5.7 and 7.5 us with 1, 2, 4 and 8 of
-    // them to a row). With many columns of B they share the staged inputs instead (48 rows of 16384 x 4096: 47, 57, 81 and 124 us).
+    // Warps take columns rather than rows while the GPU has room for the CTAs, two to an SM (head of 16384 x 768, 1 row: 6.8, 6.2,
+    // 5.7 and 7.5 us with 1, 2, 4 and 8 of them to a row). With many columns of B they share the staged inputs instead (48 rows of
+    // 16384 x 4096: 47, 57, 81 and 124 us).
     sp.k_warps = 1;
     while (NT <= 2 && sp.k_warps < kWarps && sp.k_warps < sp.chunks && (p.w.n * sp.k_warps * 2 + kWarps * MT * 16 - 1) / (kWarps * MT * 16) <= (size_t)ctx->sm_count * 2)
         sp.k_warps *= 2;

@@ -287,7 +287,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 5 : 1) token_logprob
                 p.top_ids[row * n + r] = k && !bad ? key_id(k) : PSSA_B200_NO_TOKEN;
                 p.top_logprobs[row * n + r] = bad ? kNan : k ? logp(key_value(k)) : -INFINITY;
             };
-            if (ctas == 1) {
+            if (ctas == 1 || bad) {  // a row with a NaN may have fewer keys than places
                 if (tid < n) put(tid, s.best[tid]);
             } else {  // a key's place is the number of better ones: its own list is in order, the others are searched
                 for (int i = tid; i < n * ctas; i += THREADS) {

@@ -148,6 +148,16 @@ def test_rows_without_a_distribution_and_bad_targets(gpu):
     assert torch.isnan(view[0, 5])
 
 
+@pytest.mark.parametrize("rows,vocab", [(1, 40000), (3, 70001), (200, 3000)])
+def test_a_row_of_almost_no_numbers_fills_its_alternatives(gpu, rows, vocab):
+    """Fewer logits that can be compared than alternatives asked for, in one CTA and in a cluster of them."""
+    import torch
+    view = torch.full((rows, vocab), float("nan"), device="cuda")
+    view[:, 5:9] = 1.0
+    got = forward(gpu, view, vocab, np.full(rows, 6, np.uint32), 20, 1.0)
+    assert (got["ids"] == P.NONE).all() and np.isnan(got["top"]).all() and np.isnan(got["logprob"]).all() and not got["rank"].any()
+
+
 @pytest.mark.parametrize("asked", ["logprob", "rank", "entropy", "stats", "top"])
 def test_each_result_alone_has_the_same_bits(gpu, asked):
     import torch
