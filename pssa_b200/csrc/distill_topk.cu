@@ -140,8 +140,8 @@ __global__ void __launch_bounds__(kThreads) distill_topk_long_kernel(DistillPara
     }
 }
 
-// eight warps read the row and one the teacher's entries; the row comes in pieces, each with a barrier of its own
-constexpr int kRowWarps = 8, kPartThreads = 32 * (kRowWarps + 1), kPieces = 4;
+// ROW_WARPS warps read the row and one the teacher's entries; the row comes in pieces, each with a barrier of its own
+constexpr int kMostWarps = 8, kPieces = 4;
 struct RestSums {  // of a CTA's unlisted ids: sums at the temperature, and at 1
     float top, ref, sum, sum1;
 };
@@ -154,10 +154,13 @@ struct Teacher {  // what one warp makes of a row's entries while the others rea
 };
 
 // where the warp of the teacher and those of the row meet
-__device__ __forceinline__ void ids_ready() { asm volatile("bar.sync 1, %0;" ::"n"(kPartThreads) : "memory"); }
+template <int THREADS>
+__device__ __forceinline__ void ids_ready() {
+    asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory");
+}
 
 // Run by one warp, the entries in steps of 32, behind its barrier with the others, who need the ids.
-template <typename T>
+template <typename T, int THREADS>
 __device__ void read_teacher(const DistillParams& p, size_t row, const T* x, uint32_t tgt, Teacher& s, bool report) {
     const int lane = threadIdx.x & 31, v = p.vocab;
     const float inv = 1.0f / p.teacher_temperature;
@@ -170,7 +173,7 @@ __device__ void read_teacher(const DistillParams& p, size_t row, const T* x, uin
         s.id[i] = entry ? id : PSSA_B200_NO_TOKEN;
     }
     if (lane < 3 && p.k + lane < PSSA_B200_MAX_TEACHER) s.id[p.k + lane] = PSSA_B200_NO_TOKEN;
-    ids_ready();
+    ids_ready<THREADS>();
     if (report && wrong) atomicExch(p.status, PSSA_B200_ERR_TOKEN);
     for (int i = lane; i < p.k; i += 32) {
         const uint32_t id = s.id[i];
@@ -221,14 +224,14 @@ __device__ void read_teacher(const DistillParams& p, size_t row, const T* x, uin
 }
 
 // A CTA holds elements [rank * each, + each) of a row, at the distance from a 16-byte boundary that they have in global memory.
-template <typename T>
-__global__ void __launch_bounds__(kPartThreads) distill_topk_kernel(DistillParams p, int ctas, int each) {
+template <typename T, int ROW_WARPS>
+__global__ void __launch_bounds__(32 * (ROW_WARPS + 1)) distill_topk_kernel(DistillParams p, int ctas, int each) {
     extern __shared__ __align__(128) unsigned char s_raw[];
     __shared__ Teacher s_teacher;
-    __shared__ float s_top[kRowWarps], s_ref[kRowWarps], s_sum[kRowWarps], s_sum1[kRowWarps];
+    __shared__ float s_top[ROW_WARPS], s_ref[ROW_WARPS], s_sum[ROW_WARPS], s_sum1[ROW_WARPS];
     __shared__ RestSums s_part;
     __shared__ __align__(8) uint64_t s_bar[kPieces];
-    constexpr int N = kVec<T>;
+    constexpr int N = kVec<T>, kRowWarps = ROW_WARPS, kPartThreads = 32 * (ROW_WARPS + 1);
     const size_t row = blockIdx.x / (unsigned)ctas;
     const int rank = blockIdx.x % (unsigned)ctas, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, v = p.vocab;
     const T* x = static_cast<const T*>(p.logits) + row * p.ld;
@@ -265,9 +268,9 @@ __global__ void __launch_bounds__(kPartThreads) distill_topk_kernel(DistillParam
     }
     const bool two = p.targets && p.temperature != 1.0f;
     if (warp == kRowWarps) {
-        read_teacher(p, row, x, has ? tgt : PSSA_B200_NO_TOKEN - 1, s_teacher, rank == 0);
+        read_teacher<T, kPartThreads>(p, row, x, has ? tgt : PSSA_B200_NO_TOKEN - 1, s_teacher, rank == 0);
     } else {
-        ids_ready();  // and the barriers
+        ids_ready<kPartThreads>();  // and the barriers
         // the sums of the ids that are not listed; at temperature 1 they serve the cross entropy too. Each warp masks the listed ids of its own share.
         SoftmaxSums<false> rest, rest1;
         auto mask = [&](auto mine) {
@@ -347,14 +350,15 @@ __global__ void __launch_bounds__(kPartThreads) distill_topk_kernel(DistillParam
         }
         return a;
     };
-    static_assert(kRowWarps == 8, "a part to a lane of eight");
+    static_assert(kRowWarps <= kMostWarps, "a part to a lane of eight");
     const int eighth = lane & 7;
-    RestSums all = join(RestSums{s_top[eighth], s_ref[eighth], s_sum[eighth], s_sum1[eighth]});
+    const RestSums no_part{-INFINITY, -FLT_MAX, 0.0f, 0.0f};
+    RestSums all = join(eighth < kRowWarps ? RestSums{s_top[eighth], s_ref[eighth], s_sum[eighth], s_sum1[eighth]} : no_part);
     const cg::cluster_group cluster = cg::this_cluster();
     if (ctas > 1) {
         if (tid == 0) s_part = all;
         cluster.sync();  // and every CTA has read the listed logits: from here on their places may be written
-        all = join(eighth < ctas ? *cluster.map_shared_rank(&s_part, eighth) : RestSums{-INFINITY, -FLT_MAX, 0.0f, 0.0f});
+        all = join(eighth < ctas ? *cluster.map_shared_rank(&s_part, eighth) : no_part);
         cluster.barrier_arrive();
     }
     // with the listed ids: everything relative to the row's maximum m, the rest's sum to its own
@@ -432,13 +436,13 @@ __global__ void __launch_bounds__(kPartThreads) distill_topk_kernel(DistillParam
                 write(with_ce);
             else
                 write(one);
-            const uint32_t id = tid < p.k ? s_teacher.id[tid] : PSSA_B200_NO_TOKEN;
-            const bool mine = id >= (uint32_t)e0 && id < (uint32_t)e1;
             const float xt_here = has && tgt >= (uint32_t)e0 && tgt < (uint32_t)e1 ? to_f32(held[tgt - e0]) : 0.0f;
             __syncthreads();  // the listed ids and the target go over what has been written
-            if (mine && s_teacher.t_at[tid] >= 0.0f) {
-                const float xe = s_teacher.x[tid];
-                float d = g * (mass * (expf(z_of(xe)) / s) - s_teacher.t_at[tid]);
+            for (int i = tid; i < p.k; i += kPartThreads) {
+                const uint32_t id = s_teacher.id[i];
+                const float t_at = s_teacher.t_at[i], xe = s_teacher.x[i];
+                if (id < (uint32_t)e0 || id >= (uint32_t)e1 || t_at < 0.0f) continue;
+                float d = g * (mass * (expf(z_of(xe)) / s) - t_at);
                 if (w_ce != 0.0f) d += w_ce * (expf(xe - m) / s1 - (id == tgt ? 1.0f : 0.0f));
                 out[id - e0] = from_f32<T>(d);
             }
@@ -452,22 +456,22 @@ __global__ void __launch_bounds__(kPartThreads) distill_topk_kernel(DistillParam
     if (ctas > 1) cluster.barrier_wait();  // no CTA leaves while its sums are read
 }
 
-template <typename T>
+template <typename T, int ROW_WARPS>
 int32_t launch_parts(pssa_b200_ctx* ctx, const DistillParams& p, int ctas) {
     // parts end on multiples of 16 bytes of the row, not of memory: rows may start anywhere
     const size_t each = ((p.vocab + ctas - 1) / ctas + kVec<T> - 1) / kVec<T> * kVec<T>, smem = (each + kVec<T>) * sizeof(T);
     static PerDeviceOnce attr;
     if (attr.need(ctx->device)) {
-        PSSA_CUDA(ctx, cudaFuncSetAttribute(distill_topk_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
+        PSSA_CUDA(ctx, cudaFuncSetAttribute(distill_topk_kernel<T, ROW_WARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
         attr.done(ctx->device);
     }
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(p.rows * ctas)), cfg.blockDim = dim3(kPartThreads), cfg.dynamicSmemBytes = smem, cfg.stream = ctx->stream;
+    cfg.gridDim = dim3((unsigned)(p.rows * ctas)), cfg.blockDim = dim3(32 * (ROW_WARPS + 1)), cfg.dynamicSmemBytes = smem, cfg.stream = ctx->stream;
     cudaLaunchAttribute at{};
     at.id = cudaLaunchAttributeClusterDimension;
     at.val.clusterDim.x = ctas, at.val.clusterDim.y = 1, at.val.clusterDim.z = 1;
     cfg.attrs = &at, cfg.numAttrs = ctas > 1;  // a launch with a cluster takes the host longer
-    PSSA_CUDA(ctx, cudaLaunchKernelEx(&cfg, distill_topk_kernel<T>, p, ctas, (int)each));
+    PSSA_CUDA(ctx, cudaLaunchKernelEx(&cfg, distill_topk_kernel<T, ROW_WARPS>, p, ctas, (int)each));
     return after_launch(ctx, "distill_topk_kernel");
 }
 
@@ -480,7 +484,12 @@ int32_t launch_distill_topk(pssa_b200_ctx* ctx, const DistillParams& p) {
         int ctas = 1;
         while (ctas < 8 && (bytes > (size_t)ctas * 66 * 1024 || (p.rows * ctas < (size_t)ctx->sm_count * 2 && bytes / (ctas * 2) >= 4096))) ctas *= 2;
         if (p.rows * ctas > 0x7fffffffull) return fail(ctx, PSSA_B200_ERR_SHAPE, "B200 distillation: too many rows; refusing launch");
-        return with_dtype(p.dtype, [&](auto t) { return launch_parts<decltype(t)>(ctx, p, ctas); });
+        // four row warps where there are enough short rows: more of them on their way (8039 x 5003 fp32 116 -> 75 us, 2000 x 16384 bf16
+        // 50 -> 43; 2000 x 32768 72 -> 77)
+        const bool small = ctas == 1 && bytes <= 32 * 1024 && p.rows > (size_t)ctx->sm_count * 8;
+        return with_dtype(p.dtype, [&](auto t) {
+            return small ? launch_parts<decltype(t), 4>(ctx, p, ctas) : launch_parts<decltype(t), kMostWarps>(ctx, p, ctas);
+        });
     }
     const size_t smem = ((size_t)p.vocab + 31) / 32 * 4;
     if (smem > 200 * 1024)

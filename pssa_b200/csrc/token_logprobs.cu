@@ -155,7 +155,7 @@ __device__ void best_of_part(const Part<T>& part, Key own, int n, LogprobShared<
 }
 
 template <typename T, int THREADS, bool TOP>
-__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 5 : 1) token_logprobs_kernel(LogprobParams p, int ctas) {
+__global__ void __launch_bounds__(THREADS, THREADS == 128 ? 10 : THREADS == 256 ? 5 : 1) token_logprobs_kernel(LogprobParams p, int ctas) {
     __shared__ LogprobShared<THREADS> s;
     constexpr int kWarps = THREADS / 32, N = kVec<T>, kAhead = 4;
     const size_t row = blockIdx.x / (unsigned)ctas;
@@ -391,12 +391,18 @@ cudaError_t launch_rows(pssa_b200_ctx* ctx, const LogprobParams& p, int ctas) {
 
 int32_t launch_token_logprobs(pssa_b200_ctx* ctx, const LogprobParams& p) {
     const size_t vecs = (size_t)p.vocab * dtype_size(p.dtype) / 16;
-    int ctas = 1;  // of a row: until the GPU has one to an SM, or a thread would have no vector left. A cluster costs 3 us (256 rows of 16384 with 5 alternatives: 8.1 us, 11.0 as pairs)
+    // CTAs of a row: until the GPU has one to an SM, or a thread would have no vector left. A cluster costs 3 us (256 rows of 16384
+    // with 5 alternatives: 8.1 us, 11.0 as pairs)
+    int ctas = 1;
     while (ctas < kMaxCtas && p.rows * ctas < (size_t)ctx->sm_count && vecs / (ctas * 2) >= 256) ctas *= 2;
     const bool few = p.rows * ctas <= (size_t)ctx->sm_count && vecs / ctas >= 2048;  // more threads, where few CTAs have long parts
+    // small CTAs where there are enough short rows: more rows on their way, and fewer threads to join for each (8000 x 1000 bf16 with 5
+    // alternatives 73 -> 37 us, 4245 x 16384 fp16 with 20 77 -> 66; 800 x 32768 32 -> 37, 2000 x 65536 61 -> 64)
+    const bool small = ctas == 1 && vecs <= 4096 && p.rows > (size_t)ctx->sm_count * 8;
     if (p.rows * ctas > 0x7fffffffull) return fail(ctx, PSSA_B200_ERR_SHAPE, "B200 log probabilities: too many rows; refusing launch");
     const cudaError_t e = with_dtype(p.dtype, [&](auto t) {
         using T = decltype(t);
+        if (small) return p.top_n ? launch_rows<T, 128, true>(ctx, p, ctas) : launch_rows<T, 128, false>(ctx, p, ctas);
         if (few) return p.top_n ? launch_rows<T, 1024, true>(ctx, p, ctas) : launch_rows<T, 1024, false>(ctx, p, ctas);
         return p.top_n ? launch_rows<T, 256, true>(ctx, p, ctas) : launch_rows<T, 256, false>(ctx, p, ctas);
     });

@@ -76,7 +76,7 @@ def check(got, x, ids, teacher, targets, g_kl, g_ce, temperature, t_temperature,
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows,vocab,k", [(1, 1, 1), (13, 5, 8), (14, 40, 40), (28, 1000, 1), (28, 1003, 17), (28, 5003, 64), (1, 16384, 32), (2, 16384, 256),
-                                          (28, 131072, 64), (300, 2000, 8), (3, 200003, 20), (14, 400003, 40)])
+                                          (28, 131072, 64), (300, 2000, 8), (3, 200003, 20), (14, 400003, 40), (1300, 300, 8), (1300, 513, 256)])
 @pytest.mark.parametrize("rest", [False, True])
 def test_loss_and_gradient_match_the_plain_form(gpu, dtype, rows, vocab, k, rest):
     rng = np.random.default_rng(rows * 3 + vocab + k)

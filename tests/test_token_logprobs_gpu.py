@@ -109,7 +109,7 @@ def check_forward(got, x, targets, top, temperature):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows,vocab,top", [(1, 1, 1), (1, 2, 3), (13, 7, 8), (12, 33, 33), (24, 255, 0), (25, 1000, 20), (12, 5003, 64),
-                                            (1, 8192, 5), (3, 16384, 20), (150, 4099, 5), (600, 1031, 10), (12, 131072, 20), (1, 200003, 64)])
+                                            (1, 8192, 5), (3, 16384, 20), (150, 4099, 5), (600, 1031, 10), (12, 131072, 20), (1, 200003, 64), (1300, 777, 10), (1300, 300, 64)])
 def test_forward_matches_the_plain_form(gpu, dtype, rows, vocab, top):
     rng = np.random.default_rng(rows * 7 + vocab)
     view, x = logits_of(rng, rows, vocab, dtype)
@@ -196,6 +196,11 @@ def test_alternatives_that_lie_in_one_thread_s_share(gpu, vocab, top):
         targets = np.full(len(x), 3, np.uint32)
         check_forward(forward(gpu, view, vocab, targets, top, 1.0), x, targets, top, 1.0)
         check_forward(forward(gpu, view[:1], vocab, targets[:1], top, 1.0), x[:1], targets[:1], top, 1.0)
+        if vocab <= 16384:  # many short rows take smaller CTAs
+            many = view.repeat(50, 1)
+            got = forward(gpu, many, vocab, np.full(len(many), 3, np.uint32), top, 1.0)
+            check_forward({k: v[:len(x)] for k, v in got.items()}, x, targets, top, 1.0)
+            assert all(np.array_equal(v, np.tile(v[:len(x)], (50,) + (1,) * (v.ndim - 1))) for v in got.values())
 
 
 # ---- gradient
