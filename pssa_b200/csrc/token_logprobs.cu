@@ -1,13 +1,18 @@
 // Log probabilities of given tokens with rank, entropy and top alternatives, and their gradient (see pssa_b200_token_logprobs_dev).
 //
-// Forward: one read of the row. Every thread keeps the running maximum, sum exp and sum exp * z of its vectors, counts the logits above the
-// target's, and remembers the lowest id of its maximum; the threads' and then the CTAs' numbers are joined in a fixed order. A few rows are split over the
-// CTAs of a cluster, which meet in distributed shared memory: one launch and no workspace whatever the shape.
+// Forward: one read of the row. Every thread keeps the running maximum, sum exp and sum exp * z of its vectors, counts the logits
+// above the target's, and remembers the vector of its maximum; the threads' and then the CTAs' numbers are joined in a fixed order.
+// A few rows are split over the CTAs of a cluster, which meet in distributed shared memory: one launch and no workspace whatever
+// the shape. 4096 x 131072 bf16: 212 us, 5.1 TB/s, bound by 83 instructions for 8 logits at 75 % of the issue slots. One row of 16384:
+// 9 us, of which the launch of the cluster, two dependent trips for the target's logit and the choice of 20 alternatives.
 //
-// Alternatives come from the same pass. The n-th best of the threads' maxima (of pairs of neighbouring threads) bounds the n-th best logit from below,
-// and no logit above the bound lies outside the n pairs that reach it: only their shares, n / pairs of the row, are read again, and what is not
-// below the bound, hardly more than n logits, is sorted. Keys are (value, lower id first) and so never equal: ties change nothing. Where more pass
-// than there is room for (logits in an order made for it), the n are drawn one by one instead.
+// Alternatives come from the same pass. The n-th best of the threads' maxima (of pairs of neighbouring threads) bounds the n-th
+// best logit from below, and no logit above the bound lies outside the n pairs that reach it: only their shares, n / pairs of the
+// row, are read again, and what is not below the bound, hardly more than n logits, is sorted. Keys are (value, lower id first) and so
+// never equal: ties change nothing. Where more pass than there is room for (logits in an order made for it), the n are drawn one by
+// one instead.
+//
+// Gradient: elementwise with the forward call's maximum and log sum, one read and one write: 4096 x 65536 bf16 in 159 us, 6.8 TB/s.
 #include <cooperative_groups.h>
 
 #include <type_traits>

@@ -165,6 +165,25 @@ def test_an_id_listed_twice_has_the_sum_of_its_entries(gpu):
         assert float((a[2] - b[2]).abs().max()) <= 1e-6
 
 
+@pytest.mark.parametrize("vocab", [1000, 16384, 400003])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_a_student_that_is_sure_of_the_listed_ids(gpu, vocab, dtype):
+    """The other ids share a mass of e^-150 and less: below fp32's range as a probability, not as a log probability, and the
+    gradient pushes it up relative to its own maximum."""
+    import torch
+    rng = np.random.default_rng(4)
+    x = rng.standard_normal((3, vocab))
+    ids = np.tile(np.array([[3, 500, 999]], np.uint32), (3, 1))
+    x[0, [3, 500, 999]] += 150
+    x[1, [3, 500, 999]] += 400
+    x[2, [3, 500, 999]] += 20
+    view = torch.from_numpy(x).to(getattr(torch, dtype)).cuda()
+    x = view.double().cpu().numpy()
+    teacher = np.log(np.array([[0.5, 0.3, 0.15]] * 3, np.float32))
+    g = np.array([1.0, -2.0, 0.5], np.float32)
+    check(distill(gpu, view, ids, teacher, None, g, None, 1.0, 1.0, True), x, ids, teacher, None, g, None, 1.0, 1.0, True, dtype)
+
+
 def test_gradient_matches_differences(gpu):
     rng = np.random.default_rng(9)
     for rest in (False, True):
