@@ -239,6 +239,7 @@ __global__ void __launch_bounds__(32 * (ROW_WARPS + 1)) distill_topk_kernel(Dist
     __shared__ float s_top[ROW_WARPS], s_ref[ROW_WARPS], s_sum[ROW_WARPS], s_sum1[ROW_WARPS];
     __shared__ RestSums s_part;
     __shared__ __align__(8) uint64_t s_bar[kPieces];
+    pdl_wait();
     constexpr int N = kVec<T>, kRowWarps = ROW_WARPS, kPartThreads = 32 * (ROW_WARPS + 1);
     const size_t row = blockIdx.x / (unsigned)ctas;
     const int rank = blockIdx.x % (unsigned)ctas, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, v = p.vocab;
@@ -473,13 +474,8 @@ int32_t launch_parts(pssa_b200_ctx* ctx, const DistillParams& p, int ctas) {
         PSSA_CUDA(ctx, cudaFuncSetAttribute(distill_topk_kernel<T, ROW_WARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
         attr.done(ctx->device);
     }
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(p.rows * ctas)), cfg.blockDim = dim3(32 * (ROW_WARPS + 1)), cfg.dynamicSmemBytes = smem, cfg.stream = ctx->stream;
-    cudaLaunchAttribute at{};
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = ctas, at.val.clusterDim.y = 1, at.val.clusterDim.z = 1;
-    cfg.attrs = &at, cfg.numAttrs = ctas > 1;  // a launch with a cluster takes the host longer
-    PSSA_CUDA(ctx, cudaLaunchKernelEx(&cfg, distill_topk_kernel<T, ROW_WARPS>, p, ctas, (int)each));
+    PSSA_CUDA(ctx, launch_dependent_cluster(distill_topk_kernel<T, ROW_WARPS>, dim3((unsigned)(p.rows * ctas)), dim3(32 * (ROW_WARPS + 1)), smem, ctx->stream,
+                                            ctas, p, ctas, (int)each));
     return after_launch(ctx, "distill_topk_kernel");
 }
 

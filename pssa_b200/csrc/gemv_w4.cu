@@ -190,6 +190,7 @@ constexpr int kMaxCols = 48;  // of B at a time
 template <typename T, int NT, int MT, int MODE>
 __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) gemv_w4_kernel(GemvW4Params p, W4Split sp) {
     extern __shared__ uint4 s_x[];
+    pdl_wait();
     constexpr int P = Mma<T>::pieces;
     constexpr uint32_t kMagic = Mma<T>::magic;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -475,6 +476,7 @@ __device__ __forceinline__ unsigned codes_of(const GroupForm& f, const float* x)
 // bf16 with zeros: 129 us, 2.6 TB/s; 141 with 16 to a lane). Bound by the instructions of the codes. w starts on 16 bytes.
 template <typename T, int LANES>
 __global__ void __launch_bounds__(kThreads) w4_quantize_groups_kernel(W4Params p, const T* __restrict__ w) {
+    pdl_wait();
     constexpr int kUnits = 4, kWords = sizeof(T) / 2;  // units of a lane; 16-byte words of a unit
     const size_t total = p.n * p.groups, at = ((size_t)blockIdx.x * kThreads + threadIdx.x) / LANES;
     const int lane = threadIdx.x % LANES;
@@ -530,6 +532,7 @@ __global__ void __launch_bounds__(kThreads) w4_quantize_groups_kernel(W4Params p
 // Groups of any length, one to a warp, read twice; and weights that start anywhere.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) w4_quantize_kernel(W4Params p, const T* __restrict__ w) {
+    pdl_wait();
     const size_t at = ((size_t)blockIdx.x * kThreads + threadIdx.x) >> 5;
     const int lane = threadIdx.x & 31;
     if (at >= p.n * p.groups) return;
@@ -556,23 +559,20 @@ int32_t launch_w4_quantize(pssa_b200_ctx* ctx, const W4Params& w, const void* sr
     const bool together = w.group <= 512 && (w.group & (w.group - 1)) == 0 && (reinterpret_cast<uintptr_t>(src) & 15) == 0;
     const size_t lanes = together ? w.group / 32 : 32, per = kThreads / lanes, blocks = (w.n * w.groups + per - 1) / per;
     if (blocks > 0x7fffffff) return fail(ctx, PSSA_B200_ERR_SHAPE, "B200 4-bit weights: too many groups; refusing launch");
-    with_dtype(dtype, [&](auto t) {
+    const cudaError_t e = with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
         const T* x = static_cast<const T*>(src);
-        const unsigned grid = (unsigned)blocks;
-        if (!together)
-            w4_quantize_kernel<<<grid, kThreads, 0, ctx->stream>>>(w, x);
-        else if (lanes == 1)
-            w4_quantize_groups_kernel<T, 1><<<grid, kThreads, 0, ctx->stream>>>(w, x);
-        else if (lanes == 2)
-            w4_quantize_groups_kernel<T, 2><<<grid, kThreads, 0, ctx->stream>>>(w, x);
-        else if (lanes == 4)
-            w4_quantize_groups_kernel<T, 4><<<grid, kThreads, 0, ctx->stream>>>(w, x);
-        else if (lanes == 8)
-            w4_quantize_groups_kernel<T, 8><<<grid, kThreads, 0, ctx->stream>>>(w, x);
-        else
-            w4_quantize_groups_kernel<T, 16><<<grid, kThreads, 0, ctx->stream>>>(w, x);
+        auto launch = [&](void (*kernel)(W4Params, const T*)) { return launch_dependent(kernel, dim3((unsigned)blocks), dim3(kThreads), 0, ctx->stream, w, x); };
+        if (!together) return launch(w4_quantize_kernel<T>);
+        switch (lanes) {
+            case 1: return launch(w4_quantize_groups_kernel<T, 1>);
+            case 2: return launch(w4_quantize_groups_kernel<T, 2>);
+            case 4: return launch(w4_quantize_groups_kernel<T, 4>);
+            case 8: return launch(w4_quantize_groups_kernel<T, 8>);
+            default: return launch(w4_quantize_groups_kernel<T, 16>);
+        }
     });
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "w4_quantize_kernel");
     return after_launch(ctx, together ? "w4_quantize_groups_kernel" : "w4_quantize_kernel");
 }
 
@@ -609,13 +609,8 @@ int32_t launch_tiles(pssa_b200_ctx* ctx, const GemvW4Params& p, int slice) {
         PSSA_CUDA(ctx, cudaFuncSetAttribute(gemv_w4_kernel<T, NT, MT, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
         attr.done(ctx->device);
     }
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(tiles * ctas), (unsigned)slices), cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = smem, cfg.stream = ctx->stream;
-    cudaLaunchAttribute at{};
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = ctas, at.val.clusterDim.y = 1, at.val.clusterDim.z = 1;
-    cfg.attrs = &at, cfg.numAttrs = ctas > 1;  // a launch with a cluster takes the host longer
-    PSSA_CUDA(ctx, cudaLaunchKernelEx(&cfg, gemv_w4_kernel<T, NT, MT, MODE>, p, sp));
+    PSSA_CUDA(ctx, launch_dependent_cluster(gemv_w4_kernel<T, NT, MT, MODE>, dim3((unsigned)(tiles * ctas), (unsigned)slices), dim3(kThreads), smem, ctx->stream,
+                                            ctas, p, sp));
     return after_launch(ctx, "gemv_w4_kernel");
 }
 }  // namespace

@@ -162,6 +162,7 @@ __device__ void best_of_part(const Part<T>& part, Key own, int n, LogprobShared<
 template <typename T, int THREADS, bool TOP>
 __global__ void __launch_bounds__(THREADS, THREADS == 128 ? 10 : THREADS == 256 ? 5 : 1) token_logprobs_kernel(LogprobParams p, int ctas) {
     __shared__ LogprobShared<THREADS> s;
+    pdl_wait();  // launched while the kernel before it ends: 2 us a call (it does not start the next one early: 256 rows took 9.4 for 7.9)
     constexpr int kWarps = THREADS / 32, N = kVec<T>, kAhead = 4;
     const size_t row = blockIdx.x / (unsigned)ctas;
     const int rank = blockIdx.x % (unsigned)ctas, tid = threadIdx.x, warp = tid >> 5;
@@ -328,6 +329,7 @@ constexpr int kGradThreads = 256, kGradAhead = 4;
 
 template <typename T>
 __global__ void __launch_bounds__(kGradThreads) token_logprobs_grad_kernel(LogprobGradParams p, unsigned spans) {
+    pdl_wait();
     constexpr int N = kVec<T>;
     const size_t row = blockIdx.x / spans;
     const int span = blockIdx.x % spans, tid = threadIdx.x, v = p.vocab;
@@ -383,13 +385,7 @@ __global__ void __launch_bounds__(kGradThreads) token_logprobs_grad_kernel(Logpr
 
 template <typename T, int THREADS, bool TOP>
 cudaError_t launch_rows(pssa_b200_ctx* ctx, const LogprobParams& p, int ctas) {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(p.rows * ctas)), cfg.blockDim = dim3(THREADS), cfg.stream = ctx->stream;
-    cudaLaunchAttribute at{};
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = ctas, at.val.clusterDim.y = 1, at.val.clusterDim.z = 1;
-    cfg.attrs = &at, cfg.numAttrs = ctas > 1;  // a launch with a cluster takes the host longer
-    return cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, THREADS, TOP>, p, ctas);
+    return launch_dependent_cluster(token_logprobs_kernel<T, THREADS, TOP>, dim3((unsigned)(p.rows * ctas)), dim3(THREADS), 0, ctx->stream, ctas, p, ctas);
 }
 
 }  // namespace
@@ -418,9 +414,11 @@ int32_t launch_token_logprobs(pssa_b200_ctx* ctx, const LogprobParams& p) {
 int32_t launch_token_logprobs_grad(pssa_b200_ctx* ctx, const LogprobGradParams& p) {
     const size_t per = (size_t)kGradThreads * kGradAhead * 16 / dtype_size(p.dtype), spans = (p.vocab + per - 1) / per;
     if (p.rows * spans > 0x7fffffffull) return fail(ctx, PSSA_B200_ERR_SHAPE, "B200 log probabilities' gradient: too many rows; refusing launch");
-    with_dtype(p.dtype, [&](auto t) {
-        token_logprobs_grad_kernel<decltype(t)><<<(unsigned)(p.rows * spans), kGradThreads, 0, ctx->stream>>>(p, (unsigned)spans);
+    const cudaError_t e = with_dtype(p.dtype, [&](auto t) {
+        return launch_dependent(token_logprobs_grad_kernel<decltype(t)>, dim3((unsigned)(p.rows * spans)), dim3(kGradThreads), 0, ctx->stream, p,
+                                (unsigned)spans);
     });
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "token_logprobs_grad_kernel");
     return after_launch(ctx, "token_logprobs_grad_kernel");
 }
 
