@@ -82,3 +82,73 @@ def test_a_head_in_4_bits_against_the_full_one(vocab, d, rows, group, captured):
         e, tol = P.logprob_grad(s64[r], int(t[r]), 1.0, stats[r].double().cpu().numpy(), float(h[r]), float(g[r]), float(g[r]), "float32")
         close(policy[r].double().cpu().numpy(), e, tol, "policy gradient")
     gpu.close()
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_inputs_that_another_stream_or_a_copy_has_just_written(captured):
+    """Each operator after a wait for another stream's kernel, and after a copy: the launch must wait for both. 30 rounds of inputs
+    that change; the results are those of the same calls with the device idle before each."""
+    import torch
+
+    import pssa_b200
+    side, other = torch.cuda.Stream(), torch.cuda.Stream()
+    gpu = pssa_b200.B200Dispatch(0, side)
+    rng = np.random.default_rng(5)
+    rows, vocab, d, k, group = 64, 8192, 256, 6, 64
+    rand = lambda *s: torch.from_numpy(rng.standard_normal(s).astype(np.float32)).cuda()  # noqa: E731
+    a, b, w, x = rand(rows, vocab), rand(rows, vocab), rand(vocab, d), rand(2, d)
+    targets = dev(rng.integers(0, vocab, rows).astype(np.uint32))
+    logits, w2 = torch.zeros_like(a), torch.zeros_like(w)
+    f = lambda *s: torch.zeros(*s, device="cuda")  # noqa: E731
+    ids, top, lp, stats, grad = torch.zeros(rows, k, dtype=torch.int32, device="cuda"), f(rows, k), f(rows), f(rows, 2), f(rows, vocab)
+    kl, dgrad, out = f(rows), f(rows, vocab), f(2, vocab)
+    codes, scales = torch.zeros(vocab, d // 2, dtype=torch.uint8, device="cuda"), f(vocab, d // group)
+    results = (ids, top, lp, stats, grad, kl, dgrad, codes, scales, out)
+    g = torch.full((rows,), 1.0 / rows, device="cuda")
+    torch.cuda.synchronize()
+
+    def step(wait):
+        def joined(write):
+            other.wait_stream(side)
+            with torch.cuda.stream(other):
+                write()
+            side.wait_stream(other)
+            wait()
+        joined(lambda: torch.mul(a, 0.5, out=logits))
+        gpu.token_logprobs_dev(logits, rows, vocab, targets, logprob=lp, stats=stats, top_n=k, top_ids=ids, top_logprobs=top)
+        wait()
+        gpu.token_logprobs_grad_dev(logits, rows, vocab, targets, stats, grad, grad_logprob=g)
+        wait()
+        logits.copy_(b)  # on the operators' stream, behind the gradient that reads it
+        wait()
+        gpu.distill_topk_dev(logits, rows, vocab, ids, top, k, kl=kl, grad_kl=g, grad_logits=dgrad, rest=True)
+        joined(lambda: torch.add(w, a[0, :d], out=w2))
+        gpu.w4_quantize_dev(w2, vocab, d, group, codes, scales)
+        wait()
+        gpu.gemv_w4_dev(x, 2, codes, scales, None, vocab, d, group, out)
+        wait()
+        a.mul_(-0.9).add_(b, alpha=0.1)
+        wait()
+
+    start = a.clone()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(30):
+            step(torch.cuda.synchronize)
+        want = [t.clone() for t in results]
+        a.copy_(start)
+        torch.cuda.synchronize()
+        if captured:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side, capture_error_mode="relaxed"):
+                step(lambda: None)
+            for _ in range(30):
+                graph.replay()
+        else:
+            for _ in range(30):
+                step(lambda: None)
+    torch.cuda.synchronize()
+    gpu.poll_status()
+    for t, e in zip(results, want):
+        assert torch.equal(t, e)
+    gpu.close()
