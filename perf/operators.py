@@ -298,10 +298,14 @@ _context = []
 
 
 def _gpu():
-    """The context that a program makes once, on its stream."""
+    """The context that a program makes once, on the stream that the program works on now."""
+    stream = torch.cuda.current_stream()
     if not _context:
         import pssa_b200
-        _context.append(pssa_b200.B200Dispatch(0, torch.cuda.current_stream()))
+        _context[:] = pssa_b200.B200Dispatch(0, stream), stream
+    elif _context[1] != stream:
+        _context[0].set_stream(stream)
+        _context[1] = stream
     return _context[0]
 
 
