@@ -593,7 +593,8 @@ int32_t pssa_b200_token_logprobs_grad_dev(pssa_b200_ctx* ctx, const void* logits
  * PSSA_B200_ERR_TOKEN in the status word and count as absent (ce NaN). ln p is held in fp32 and is -inf below its range.
  * Masked student logits (-inf) under a teacher's mass give kl = +inf and a finite gradient; a row of masked ids only gives kl
  * (where the teacher has mass) and ce +inf and a zero gradient. A row with a NaN or +inf gives NaN. A row whose gradient
- * weights are all zero gets a zero gradient whatever its logits hold.
+ * weights are all zero gets a zero gradient whatever its logits hold. A teacher's entry that is NaN, or +inf at its temperature,
+ * makes its row's kl NaN, and the gradient too where grad_kl is not zero; ce and its gradient do not depend on the teacher.
  */
 int32_t pssa_b200_distill_topk_dev(pssa_b200_ctx* ctx, const void* logits, int32_t dtype, size_t rows, size_t vocab, size_t ld,
                                    float temperature, const uint32_t* teacher_ids, const float* teacher, size_t k,

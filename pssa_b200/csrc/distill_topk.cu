@@ -42,6 +42,12 @@ __device__ __forceinline__ T block_reduce(T v, T* scratch, F op) {
     return v;
 }
 
+// a teacher's entry at its temperature; one that is +inf is no number like a NaN
+__device__ __forceinline__ float teacher_entry(const DistillParams& p, size_t row, int i) {
+    const float q = p.teacher[row * p.k + i] * (1.0f / p.teacher_temperature);
+    return q < INFINITY ? q : kNan;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads) distill_topk_long_kernel(DistillParams p) {
     extern __shared__ unsigned s_bits[];
@@ -69,7 +75,7 @@ __global__ void __launch_bounds__(kThreads) distill_topk_long_kernel(DistillPara
     const uint32_t id = tid < p.k ? p.teacher_ids[row * p.k + tid] : PSSA_B200_NO_TOKEN;
     const bool entry = id < (uint32_t)v;
     bool wrong = !entry && id != PSSA_B200_NO_TOKEN;
-    const float q = entry ? p.teacher[row * p.k + tid] * (1.0f / p.teacher_temperature) : -INFINITY;
+    const float q = entry ? teacher_entry(p, row, tid) : -INFINITY;
     float t, log_t = q, r = 0.0f;
     if (p.rest) {
         t = entry ? expf(q) : 0.0f;
@@ -134,13 +140,15 @@ __global__ void __launch_bounds__(kThreads) distill_topk_long_kernel(DistillPara
         if (!zero) {
             const float a = to_f32(x[i]);
             const bool listed = s_bits[i >> 5] >> (i & 31) & 1;
-            if (listed)
-                d = g_kl * mass * (expf((a - m) * inv_t) / s);
-            else
-                d = su > 0.0f ? g_kl * (expf((a - mu) * inv_t) / su * (p.rest ? mass * p_rest - r : mass * p_rest)) : 0.0f;
-            if (listed)
-                for (int j = 0; j < p.k; ++j)
-                    if (s_id[j] == (unsigned)i) d -= g_kl * s_t[j];
+            if (w_kl != 0.0f) {  // a teacher that is no number does not enter without a weight
+                if (listed)
+                    d = g_kl * mass * (expf((a - m) * inv_t) / s);
+                else
+                    d = su > 0.0f ? g_kl * (expf((a - mu) * inv_t) / su * (p.rest ? mass * p_rest - r : mass * p_rest)) : 0.0f;
+                if (listed)
+                    for (int j = 0; j < p.k; ++j)
+                        if (s_id[j] == (unsigned)i) d -= g_kl * s_t[j];
+            }
             if (w_ce != 0.0f) d += w_ce * (expf(a - m) / s1 - (i == (int)tgt ? 1.0f : 0.0f));
             if (bad) d = kNan;
         }
@@ -153,10 +161,11 @@ constexpr int kMostWarps = 8, kPieces = 4;
 struct RestSums {  // of a CTA's unlisted ids: sums at the temperature, and at 1
     float top, ref, sum, sum1;
 };
+constexpr float kNotFirst = -1.0f;
 struct Teacher {  // what one warp makes of a row's entries while the others read the row
     alignas(16) uint32_t id[PSSA_B200_MAX_TEACHER];  // PSSA_B200_NO_TOKEN: absent, and behind the last up to a multiple of 4
     float t[PSSA_B200_MAX_TEACHER], log_t[PSSA_B200_MAX_TEACHER], x[PSSA_B200_MAX_TEACHER];
-    float t_at[PSSA_B200_MAX_TEACHER];   // the id's whole mass at its first entry, -1 at others of it
+    float t_at[PSSA_B200_MAX_TEACHER];   // the id's whole mass at its first entry, kNotFirst at others of it: the mass may be a NaN
     float x_max, rest, mass;             // of the listed logits; 1 - sum t, with DISTILL_REST; sum t + rest
     int bad, target;                     // a listed logit is no number; the target's entry or -1
 };
@@ -171,7 +180,6 @@ __device__ __forceinline__ void ids_ready() {
 template <typename T, int THREADS>
 __device__ void read_teacher(const DistillParams& p, size_t row, const T* x, uint32_t tgt, Teacher& s, bool report) {
     const int lane = threadIdx.x & 31, v = p.vocab;
-    const float inv = 1.0f / p.teacher_temperature;
     float q_max = -INFINITY, x_max = -INFINITY;
     bool wrong = false, bad = false, any = false;
     for (int i = lane; i < p.k; i += 32) {
@@ -186,7 +194,7 @@ __device__ void read_teacher(const DistillParams& p, size_t row, const T* x, uin
     for (int i = lane; i < p.k; i += 32) {
         const uint32_t id = s.id[i];
         const bool entry = id != PSSA_B200_NO_TOKEN;
-        const float q = entry ? p.teacher[row * p.k + i] * inv : -INFINITY, xe = entry ? to_f32(x[id]) : -INFINITY;
+        const float q = entry ? teacher_entry(p, row, i) : -INFINITY, xe = entry ? to_f32(x[id]) : -INFINITY;
         bad |= xe != xe;
         s.x[i] = xe, s.log_t[i] = q;
         q_max = fmaxf(q_max, q != q ? INFINITY : q), x_max = fmaxf(x_max, xe);
@@ -224,7 +232,7 @@ __device__ void read_teacher(const DistillParams& p, size_t row, const T* x, uin
             if (o.z == id) first = first && j + 2 >= i, t_at += s.t[j + 2];
             if (o.w == id) first = first && j + 3 >= i, t_at += s.t[j + 3];
         }
-        s.t_at[i] = first ? t_at : -1.0f;
+        s.t_at[i] = first ? t_at : kNotFirst;
         if (first && id == tgt) target = i;
     }
     x_max = warp_max(x_max), mass = warp_sum(mass) + rest, bad = __any_sync(0xffffffffu, bad), target = __reduce_max_sync(0xffffffffu, target);
@@ -377,7 +385,7 @@ __global__ void __launch_bounds__(32 * (ROW_WARPS + 1)) distill_topk_kernel(Dist
     auto z_of = [&](float a) { return empty ? -INFINITY : (a - m) * inv_t; };
     float listed = 0.0f, listed1 = 0.0f;  // each warp for itself
     for (int i = lane; i < p.k; i += 32)
-        if (s_teacher.t_at[i] >= 0.0f) {
+        if (s_teacher.t_at[i] != kNotFirst) {
             listed += expf(z_of(s_teacher.x[i]));
             if (two) listed1 += expf(empty ? -INFINITY : s_teacher.x[i] - m);
         }
@@ -401,7 +409,7 @@ __global__ void __launch_bounds__(32 * (ROW_WARPS + 1)) distill_topk_kernel(Dist
         const bool zero = (w_kl == 0.0f && w_ce == 0.0f) || (empty && !bad);
         const float g = w_kl * inv_t;
         // an unlisted id: its share of the rest, times a, and its probability at temperature 1
-        const float a = all.sum > 0.0f ? g * (p.rest ? mass * p_rest - r : mass * p_rest) / all.sum : 0.0f;
+        const float a = w_kl != 0.0f && all.sum > 0.0f ? g * (p.rest ? mass * p_rest - r : mass * p_rest) / all.sum : 0.0f;
         const float a1 = w_ce * ex2(to_m * kLog2e) / s1, both = two ? a : a + a1;
         const float nref = -all.ref;
         T* out = static_cast<T*>(p.grad) + row * p.ld_grad + e0;
@@ -450,8 +458,8 @@ __global__ void __launch_bounds__(32 * (ROW_WARPS + 1)) distill_topk_kernel(Dist
             for (int i = tid; i < p.k; i += kPartThreads) {
                 const uint32_t id = s_teacher.id[i];
                 const float t_at = s_teacher.t_at[i], xe = s_teacher.x[i];
-                if (id < (uint32_t)e0 || id >= (uint32_t)e1 || t_at < 0.0f) continue;
-                float d = g * (mass * (expf(z_of(xe)) / s) - t_at);
+                if (id < (uint32_t)e0 || id >= (uint32_t)e1 || t_at == kNotFirst) continue;
+                float d = w_kl != 0.0f ? g * (mass * (expf(z_of(xe)) / s) - t_at) : 0.0f;
                 if (w_ce != 0.0f) d += w_ce * (expf(xe - m) / s1 - (id == tgt ? 1.0f : 0.0f));
                 out[id - e0] = from_f32<T>(d);
             }
