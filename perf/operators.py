@@ -327,10 +327,11 @@ def _own(st):
                              targets=st["targets"] if c["ce"] else None, ce=st["ce"], grad_ce=st["g_ce"], grad_logits=st["grad"],
                              temperature=c["temperature"], rest=c["rest"])
         return st["kl"], st["ce"], st["grad"]
+    group = min(c["group"], -(-c["k"] // 128) * 128)  # one group of a narrow matrix: no wider than the call takes it
     if c["op"] == "quantize":
-        gpu.w4_quantize_dev(st["w"], c["n"], c["k"], c["group"], st["codes"], st["scales"], st["zeros"])
+        gpu.w4_quantize_dev(st["w"], c["n"], c["k"], group, st["codes"], st["scales"], st["zeros"])
         return st["codes"], st["scales"], st["zeros"]
-    gpu.gemv_w4_dev(st["x"], c["rows"], st["codes"], st["scales"], st["zeros"], c["n"], c["k"], c["group"], st["out"])
+    gpu.gemv_w4_dev(st["x"], c["rows"], st["codes"], st["scales"], st["zeros"], c["n"], c["k"], group, st["out"])
     return st["out"]
 
 
