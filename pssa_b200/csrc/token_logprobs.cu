@@ -76,8 +76,8 @@ struct Part {
     // this thread's single element: its id, or -1
     __device__ int single() const {
         if (first && (int)threadIdx.x < head) return threadIdx.x;
-        const int i = tail0 + (int)threadIdx.x - kVec<T>;  // behind the heads' threads
-        return last && (int)threadIdx.x >= kVec<T> && i < n ? i : -1;
+        const int i = (int)threadIdx.x - kVec<T>;  // behind the heads' threads
+        return last && i >= 0 && i < n - tail0 ? tail0 + i : -1;
     }
 };
 
@@ -316,7 +316,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 128 ? 10 : THREADS == 256 
                     }
                     if (place < n) put(place, k);
                 }
-                for (int r = v + tid; r < n; r += THREADS) put(r, 0);  // fewer ids than places
+                for (int r = min(v, n) + tid; r < n; r += THREADS) put(r, 0);  // fewer ids than places
             }
         }
     }
@@ -376,10 +376,11 @@ __global__ void __launch_bounds__(kGradThreads) token_logprobs_grad_kernel(Logpr
     }
     auto single = [&](int i) { out[i] = from_f32<T>(zero ? 0.0f : one(to_f32(x[i])) + ((unsigned)i == t ? g : 0.0f)); };
     if (!together) {
-        for (int i = span * kGradThreads * kGradAhead * N + tid; i < min((span + 1) * kGradThreads * kGradAhead * N, v); i += kGradThreads) single(i);
+        const int i0 = span * kGradThreads * kGradAhead * N, n = min(kGradThreads * kGradAhead * N, v - i0);
+        for (int i = tid; i < n; i += kGradThreads) single(i0 + i);
     } else if (span == 0) {
         if (tid < head) single(tid);
-        if (tail0 + tid < v) single(tail0 + tid);
+        if (tid < v - tail0) single(tail0 + tid);
     }
 }
 

@@ -62,3 +62,45 @@ def test_a_teacher_that_is_no_number_leaves_the_cross_entropy(gpu, vocab, rest, 
     for r in range(rows):
         w = P.distill(x[r], ids[r], fine[r].astype(np.float64), temperature, t_temperature, rest, int(targets[r]), 0.0, float(g_ce[r]), "float32")
         close(grad2[r].double().cpu().numpy(), w["grad"], w["tol_g"], f"gradient of the cross entropy {r}")
+
+
+@pytest.mark.parametrize("shift,gshift", [(0, 0), (1, 1), (0, 1)])
+def test_a_vocabulary_just_below_2_31(gpu, shift, gshift):
+    """Every index of the last elements and of what lies behind them is near the end of 32 bits. The bulk is 0, so that its sums are
+    whole numbers below 2^24 in every thread whose reference is 0. It is a peak's in the warps that start with one: the one with the
+    elements behind the last vector, and the one at the row's middle, where a CTA starts. These are 64 of 8192 threads (8 CTAs of
+    1024), and each rounds its 2^31 / 8192 / 2 sums of pairs by at most 2^-24 of a running sum that is half the last one on
+    average: 2^17 / 2 * 64 / 8192 = 512 times 2^-24 of the whole. The joins are at most 40 roundings more, and the logarithm of
+    2^31 has steps of 2^-19. An entropy is ls less ent / sum, of about 2: e from the first and 2 (e + e) from the second."""
+    import torch
+    v, top = (1 << 31) - 1, 5
+    buf, out = torch.zeros(v + 80, dtype=torch.bfloat16, device="cuda"), torch.full((v + 80,), 5.0, dtype=torch.bfloat16, device="cuda")
+    x, grad = buf[shift:shift + v].view(1, v), out[gshift:gshift + v].view(1, v)
+    peaks = [v - 1, v - 2, v // 2, 1 << 30]
+    x[0, peaks] = torch.tensor([2.0, 1.5, 1.0, 0.5], dtype=torch.bfloat16, device="cuda")
+    buf[shift + v:] = 50.0  # behind the row
+    target = dev(np.array([v - 1], np.uint32))
+    lp, h, stats, rank = (torch.zeros(1, device="cuda"), torch.zeros(1, device="cuda"), torch.zeros(1, 2, device="cuda"),
+                          torch.zeros(1, dtype=torch.int32, device="cuda"))
+    ids, tops = torch.zeros(top + 2, dtype=torch.int32, device="cuda"), torch.full((top + 2,), 7.0, device="cuda")
+    ids[-1] = 77
+    gpu.token_logprobs_dev(x, 1, v, target, logprob=lp, rank=rank, entropy=h, stats=stats, top_n=top, top_ids=ids[:top], top_logprobs=tops[:top], ld=v)
+    g = torch.ones(1, device="cuda")
+    gpu.token_logprobs_grad_dev(x, 1, v, target, stats, grad, grad_logprob=g, ld=v, ld_grad=v)
+    torch.cuda.synchronize()
+    gpu.poll_status()
+    w = np.exp(np.array([2.0, 1.5, 1.0, 0.5]))
+    total = (v - 4) + w.sum()
+    tol = (512 + 40) * P.U + 2.0 ** -19
+    assert abs(float(lp) - (2.0 - np.log(total))) <= tol and int(rank) == 1
+    assert abs(float(h) - (np.log(total) - (w * np.log(w)).sum() / total)) <= 5 * tol
+    assert float(stats[0, 0]) == 2.0 and abs(float(stats[0, 1]) - (np.log(total) - 2.0)) <= tol
+    assert ids.cpu().tolist() == peaks + [0, 0, 77] and float(tops[-1]) == 7.0
+    # the gradient: -1 / total in the bulk, 1 - p at the target; what is behind the row stays
+    for i, a in zip(peaks, w):
+        want = float(i == v - 1) - a / total
+        assert abs(float(grad[0, i]) - want) <= 2.0 ** -8 * abs(want) + tol * a / total
+    grad[0, peaks] = float(grad[0, 0])
+    assert abs(float(grad[0, 0]) + 1 / total) <= (2.0 ** -8 + tol) / total
+    assert float(grad.min()) == float(grad.max()) == float(grad[0, 0])
+    assert bool((out[:gshift] == 5.0).all()) and bool((out[gshift + v:] == 5.0).all())
