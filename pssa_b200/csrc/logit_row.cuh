@@ -124,28 +124,43 @@ __device__ __forceinline__ float vector_max(uint4 v, const float (&x)[kVec<T>]) 
 // lose nothing. `ref` is never below the lowest finite number: a row of that value alone is a distribution like any other, a row of
 // -inf is none. A difference is formed before it is scaled, so that logits far from zero lose nothing. A NaN or +inf makes `sum` a
 // NaN, or `top` infinite.
-template <bool ENTROPY, bool WHERE = false>
+// APART: the logit that `ref` was taken from stays out of the sums, where it would be 1 (`apart`). Of a row that is sure of one id the
+// sum is then what that id leaves, and ln(1 + sum) is right to its last bits however small it is: with the 1 in it, a row whose
+// entropy is 0.004 lost 4e-5 of it.
+template <bool ENTROPY, bool WHERE = false, bool APART = false>
 struct SoftmaxSums {
     float top = -INFINITY, ref = -FLT_MAX, lim = -FLT_MAX;
     F2 sum = {0}, ent = {0};  // sum 2^t, sum 2^t t with t = (x - ref) c; 64 bits of 0 are a pair of zeros
     int where = -1;           // WHERE: the first vector that holds `top`
+    bool apart = false;
 
     __device__ __forceinline__ void start(float m, float c) {
         if (m > ref) ref = m, lim = m + 4.0f / c;
     }
     __device__ __forceinline__ void raise(float m, float c) {
+        if (APART && apart) sum = add2(sum, pair(1.0f, 0.0f));
         const float d = fmaxf((ref - m) * c, -1e4f), f = ex2(d);
         const F2 f2 = pair(f, f);
         if (ENTROPY) ent = mul2(f2, fma2(pair(d, d), sum, ent));
         sum = mul2(f2, sum);
         start(m, c);
     }
-    // N elements whose largest is m
-    template <int N>
-    __device__ __forceinline__ void add(const float (&x)[N], float m, int at, float c) {
+    // N elements whose largest is m. FIRST: they are among those that the warp started from, of which none is above `ref`. With APART, x
+    // comes back without the one that stays out.
+    template <bool FIRST = false, int N>
+    __device__ __forceinline__ void add(float (&x)[N], float m, int at, float c) {
         if (WHERE) where = m > top ? at : where;
         top = fmaxf(top, m);
-        if (m > lim) raise(m, c);
+        if (FIRST ? APART && m == ref && !apart : m > lim) {
+            if (!FIRST) raise(m, c);
+            if (APART) {
+                apart = true;
+                bool out = false;
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                    if (x[i] == m && !out) x[i] = -INFINITY, out = true;
+            }
+        }
         const F2 nref = pair(-ref, -ref), c2 = pair(c, c);
 #pragma unroll
         for (int i = 0; i < N; i += 2) {
@@ -159,7 +174,14 @@ struct SoftmaxSums {
     }
     __device__ __forceinline__ void add1(float x, float c) {
         top = fmaxf(top, x);
-        if (x > lim) raise(x, c);
+        if (x > lim) {
+            raise(x, c);
+            apart = false;
+        }
+        if (APART && x == ref && !apart) {
+            apart = true;
+            return;
+        }
         const float t = (x - ref) * c, w = ex2(t);
         sum = add2(sum, pair(w, 0.0f));
         if (ENTROPY) ent = fma2(pair(w, 0.0f), pair(fmaxf(t, -200.0f), 0.0f), ent);

@@ -32,13 +32,20 @@ constexpr int kMaxCtas = 8;  // of a cluster
 struct RowPart {  // a CTA's numbers for its cluster
     float top, ref, sum, ent;
     unsigned above;
+    bool apart;  // of one logit equal to `ref`: it is not in `sum`
 };
+// `sum` relative to `to` >= `ref`, where the logit of `ref` is 1 no longer
+__device__ __forceinline__ void raise_to(RowPart& p, float to, float c) {
+    if (p.apart && p.ref < to) p.sum += 1.0f, p.apart = false;
+    rebase(p.ref, to, c, p.sum, p.ent);
+    p.ref = to;
+}
 
 template <int THREADS>
 struct LogprobShared {
     RowPart part, parts[kMaxCtas];
     float f[3][THREADS / 32];
-    unsigned u[THREADS / 32];
+    unsigned u[THREADS / 32];  // how many are above; the highest bit: one stays apart
     Key bound, wide[THREADS / 32];
     int candidates;
     Key pairs[THREADS / 2];
@@ -174,17 +181,17 @@ __global__ void __launch_bounds__(THREADS, THREADS == 128 ? 10 : THREADS == 256 
     const bool has = t < (uint32_t)v, none = t == PSSA_B200_NO_TOKEN;
     const float xt = has ? to_f32(x[t]) : INFINITY;
 
-    SoftmaxSums<true, TOP> sums;
+    SoftmaxSums<true, TOP, true> sums;
     unsigned above = 0;
-    auto take = [&](uint4 raw, int at) {
+    auto take = [&](uint4 raw, int at, auto first) {
         float f[N];
         unpack<T>(raw, f);
         const float m = vector_max<T>(raw, f);
-        sums.add(f, m, at, c);
         if (m > xt) {
 #pragma unroll
             for (int i = 0; i < N; ++i) above += f[i] > xt;
         }
+        sums.template add<decltype(first)::value>(f, m, at, c);
     };
     const int one = part.single();
     const float single = one >= 0 ? to_f32(x[one]) : -INFINITY;
@@ -205,7 +212,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 128 ? 10 : THREADS == 256 
         sums.start(warp_max(m), c);
 #pragma unroll
         for (int i = 0; i < kAhead; ++i)
-            if (at + i * THREADS < part.v1) take(raw[i], at + i * THREADS);
+            if (at + i * THREADS < part.v1) take(raw[i], at + i * THREADS, std::true_type());
         at += kAhead * THREADS;
     }
     for (; at + (kAhead - 1) * THREADS < part.v1; at += kAhead * THREADS) {
@@ -213,9 +220,9 @@ __global__ void __launch_bounds__(THREADS, THREADS == 128 ? 10 : THREADS == 256 
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) raw[i] = part.vec[at + i * THREADS];
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) take(raw[i], at + i * THREADS);
+        for (int i = 0; i < kAhead; ++i) take(raw[i], at + i * THREADS, std::false_type());
     }
-    for (; at < part.v1; at += THREADS) take(part.vec[at], at);
+    for (; at < part.v1; at += THREADS) take(part.vec[at], at, std::false_type());
     Key own = 0;  // the thread's best logit
     if (TOP) {
         if (const int w = sums.where >= 0 ? sums.where : part.v0 + tid; w < part.v1) {  // without one above -inf, the lowest of its ids
@@ -239,7 +246,10 @@ __global__ void __launch_bounds__(THREADS, THREADS == 128 ? 10 : THREADS == 256 
     // the CTA's numbers
     const float ref = block_reduce<THREADS>(sums.ref, s.f[0], [](float a, float b) { return fmaxf(a, b); });
     const float top = block_reduce<THREADS>(sums.top, s.f[0], [](float a, float b) { return fmaxf(a, b); });
-    float sum = sums.total(), ent = sums.entropy_total();
+    float ent = sums.entropy_total();
+    const unsigned apart = __ballot_sync(0xffffffffu, sums.apart && sums.ref == ref);  // the first of the warp's stays apart
+    const bool counts = sums.apart && (sums.ref < ref || (apart & ((1u << (tid & 31)) - 1)));
+    float sum = sums.total() + (counts ? 1.0f : 0.0f);
     rebase(sums.ref, ref, c, sum, ent);
 #pragma unroll
     for (int m = 16; m > 0; m >>= 1) {
@@ -247,12 +257,13 @@ __global__ void __launch_bounds__(THREADS, THREADS == 128 ? 10 : THREADS == 256 
         ent += __shfl_xor_sync(0xffffffffu, ent, m);
         above += __shfl_xor_sync(0xffffffffu, above, m);
     }
-    if ((tid & 31) == 0) s.f[1][warp] = sum, s.f[2][warp] = ent, s.u[warp] = above;
+    if ((tid & 31) == 0) s.f[1][warp] = sum, s.f[2][warp] = ent, s.u[warp] = above | (apart ? 0x80000000u : 0);
     __syncthreads();
     if (tid == 0) {
         sum = ent = 0.0f, above = 0;
-        for (int i = 0; i < kWarps; ++i) sum += s.f[1][i], ent += s.f[2][i], above += s.u[i];
-        s.part = RowPart{top, ref, sum, ent, above};
+        unsigned all = 0;
+        for (int i = 0; i < kWarps; ++i) sum += s.f[1][i], ent += s.f[2][i], above += s.u[i] & 0x7fffffffu, all += s.u[i] >> 31;
+        s.part = RowPart{top, ref, all > 1 ? sum + (float)(all - 1) : sum, ent, above, all > 0};
     }
     if (TOP) best_of_part<T, THREADS>(part, own, p.top_n, s);
     // the cluster's
@@ -272,19 +283,20 @@ __global__ void __launch_bounds__(THREADS, THREADS == 128 ? 10 : THREADS == 256 
         for (int i = 1; i < ctas; ++i) {
             RowPart o = s.parts[i];
             const float to = fmaxf(all.ref, o.ref);
-            rebase(all.ref, to, c, all.sum, all.ent);
-            rebase(o.ref, to, c, o.sum, o.ent);
-            all.ref = to, all.top = fmaxf(all.top, o.top), all.sum += o.sum, all.ent += o.ent, all.above += o.above;
+            raise_to(all, to, c);
+            raise_to(o, to, c);
+            all.top = fmaxf(all.top, o.top), all.sum += o.sum + (all.apart && o.apart ? 1.0f : 0.0f), all.ent += o.ent, all.above += o.above;
+            all.apart |= o.apart;
         }
         const bool bad = all.sum != all.sum || all.top == INFINITY, empty = all.top == -INFINITY;
-        if (!empty) rebase(all.ref, all.top, c, all.sum, all.ent);
-        const float ls = empty ? 0.0f : logf(all.sum);
+        if (!empty) raise_to(all, all.top, c);
+        const float ls = empty ? 0.0f : all.apart ? log1pf(all.sum) : logf(all.sum);
         auto logp = [&](float a) { return bad ? kNan : empty ? -INFINITY : (a - all.top) * inv_t - ls; };
         if (tid == 0) {
             if (!has && !none) atomicExch(p.status, PSSA_B200_ERR_TOKEN);
             if (p.logprob) p.logprob[row] = none ? 0.0f : has ? logp(xt) : kNan;
             if (p.rank) p.rank[row] = bad || !has ? 0 : all.above + 1;
-            if (p.entropy) p.entropy[row] = bad ? kNan : empty ? 0.0f : ls - kLn2 * (all.ent / all.sum);
+            if (p.entropy) p.entropy[row] = bad ? kNan : empty ? 0.0f : ls - kLn2 * (all.ent / (all.apart ? 1.0f + all.sum : all.sum));
             if (p.stats) p.stats[2 * row] = bad ? kNan : all.top, p.stats[2 * row + 1] = bad ? kNan : ls;
         }
         if (TOP) {

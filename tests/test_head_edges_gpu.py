@@ -104,3 +104,35 @@ def test_a_vocabulary_just_below_2_31(gpu, shift, gshift):
     assert abs(float(grad[0, 0]) + 1 / total) <= (2.0 ** -8 + tol) / total
     assert float(grad.min()) == float(grad.max()) == float(grad[0, 0])
     assert bool((out[:gshift] == 5.0).all()) and bool((out[gshift + v:] == 5.0).all())
+
+
+def sure_rows(rng, rows, vocab, dtype):
+    """Rows with one id far above the others, which share 1e-1 to 1e-12 of the mass; the id lies at a row's ends and between them."""
+    import torch
+    x = rng.standard_normal((rows, vocab)) * 2
+    best = np.array([(0, vocab - 1, vocab // 2, 1, min(8, vocab - 1), vocab // 3, vocab - 2, (5 * vocab) // 7)[r % 8] for r in range(rows)])
+    x[np.arange(rows), best] = np.log(np.exp(x).sum(1)) + rng.uniform(2.3, 28, rows)
+    view = torch.from_numpy(x).to(getattr(torch, dtype)).cuda()
+    return view, view.double().cpu().numpy(), best
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("rows,vocab,top", [(8, 40, 2), (16, 1000, 0), (1, 16384, 20), (8, 16384, 5), (16, 70001, 0), (1, 131072, 3), (200, 5003, 1), (1400, 600, 4)])
+@pytest.mark.parametrize("temperature", [1.0, 0.7])
+def test_a_row_that_is_sure_of_one_id_keeps_its_small_numbers(gpu, dtype, rows, vocab, top, temperature):
+    """Entropy, log sum and the best id's log probability come from what the other ids leave, each of whose terms has an argument of
+    3 roundings, an exponential of 2 more, `adds` sums and a logarithm or a quotient of 2: relative to the result, however small."""
+    from test_token_logprobs_gpu import forward
+    view, x, best = sure_rows(np.random.default_rng(vocab + rows), rows, vocab, dtype)
+    got = forward(gpu, view, vocab, best.astype(np.uint32), top, temperature)
+    for r in range(rows):
+        z = (x[r] - x[r].max()) / temperature
+        assert z.argmax() == best[r]
+        others = np.delete(z, best[r])
+        rest = np.exp(others).sum()
+        l, h = np.log1p(rest), np.log1p(rest) + (np.exp(others) * -others).sum() / (1 + rest)
+        tol = P.U * (3 * -others.min() + 2 * P.adds(vocab) + 20)
+        for name, a, want in (("log sum", got["stats"][r, 1], l), ("log probability", got["logprob"][r], -l), ("entropy", got["entropy"][r], h),
+                              *([("best", got["top"][r, 0], -l)] if top else [])):
+            assert abs(float(a) - want) <= tol * abs(want) + 2.0 ** -149, (name, r, float(a), want)
+        assert got["rank"][r] == 1
