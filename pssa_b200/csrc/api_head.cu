@@ -1,5 +1,6 @@
 // extern "C" entry points of the operators on a head's weights and logits: products with 4-bit weights, log probabilities, distillation.
 #include <cmath>
+#include <initializer_list>
 
 #include "bounds.hpp"
 #include "element.cuh"
@@ -35,6 +36,13 @@ int32_t invalid(pssa_b200_ctx* ctx, const char* what, const char* why) {
 
 bool known_dtype(int32_t dtype) { return dtype >= PSSA_B200_F32 && dtype <= PSSA_B200_F16; }
 bool aligned(const void* p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+
+// arrays of u32 or fp32, each of which may be absent
+bool words(std::initializer_list<const void*> arrays) {
+    for (const void* p : arrays)
+        if (!aligned(p, 4)) return false;
+    return true;
+}
 
 // [rows, cols] elements with a row pitch: its extent in bytes
 int32_t pitched(pssa_b200_ctx* ctx, const char* what, const char* array, size_t rows, size_t cols, size_t ld, int32_t dtype, const void* p, size_t* bytes) {
@@ -154,6 +162,7 @@ int32_t pssa_b200_token_logprobs_dev(pssa_b200_ctx* ctx, const void* logits, int
         return invalid(ctx, what, "alternatives need top_n, top_ids and top_logprobs, all or none");
     if ((logprob || rank) && !targets) return invalid(ctx, what, "log probability and rank need targets");
     if (!logprob && !rank && !entropy && !stats && top_n == 0) return invalid(ctx, what, "no output is asked for");
+    if (!words({targets, logprob, rank, entropy, stats, top_ids, top_logprobs})) return invalid(ctx, what, "an array is not aligned to its elements");
     const OnDevice on(ctx->device);
     PSSA_CUDA(ctx, on.error);
     LogprobParams p{};
@@ -174,6 +183,7 @@ int32_t pssa_b200_token_logprobs_grad_dev(pssa_b200_ctx* ctx, const void* logits
     if (!grad_logits || !stats) return invalid(ctx, what, "null gradient or stats");
     if (grad_logprob && !targets) return invalid(ctx, what, "a weight of the log probability needs targets");
     if (grad_entropy && !entropy) return invalid(ctx, what, "a weight of the entropy needs the entropy");
+    if (!words({targets, stats, entropy, grad_logprob, grad_entropy})) return invalid(ctx, what, "an array is not aligned to its elements");
     if ((rc = gradient_place(ctx, what, logits, bytes, ld, grad_logits, ld_grad, rows, vocab, dtype))) return rc;
     const OnDevice on(ctx->device);
     PSSA_CUDA(ctx, on.error);
@@ -207,6 +217,7 @@ int32_t pssa_b200_distill_topk_dev(pssa_b200_ctx* ctx, const void* logits, int32
     if (grad_logits && !grad_kl && !grad_ce) return invalid(ctx, what, "a gradient needs the weight of a loss");
     if (!grad_logits && (grad_kl || grad_ce)) return invalid(ctx, what, "weights of losses without a gradient");
     if (!kl && !ce && !grad_logits) return invalid(ctx, what, "no output is asked for");
+    if (!words({teacher_ids, teacher, targets, kl, ce, grad_kl, grad_ce})) return invalid(ctx, what, "an array is not aligned to its elements");
     if (grad_logits && (rc = gradient_place(ctx, what, logits, bytes, ld, grad_logits, ld_grad, rows, vocab, dtype))) return rc;
     const OnDevice on(ctx->device);
     PSSA_CUDA(ctx, on.error);
