@@ -24,14 +24,6 @@ def _ptr(x):
     raise TypeError(f"cannot take a pointer of {type(x)}")
 
 
-def _addr(x):
-    """`_ptr` as a plain number, which ctypes passes as it is: a decode step's calls have a dozen of them and take 10 us."""
-    try:
-        return x.data_ptr()
-    except AttributeError:
-        return None if x is None else _ptr(x).value
-
-
 def _host(a, name, shape=None):
     if not isinstance(a, np.ndarray) or a.dtype != np.float32 or not a.flags["C_CONTIGUOUS"]:
         raise TypeError(f"{name} must be a C-contiguous float32 numpy array")
@@ -42,6 +34,17 @@ def _host(a, name, shape=None):
 
 _DTYPES = {"float32": N.F32, "bfloat16": N.BF16, "float16": N.F16}
 _TORCH_DTYPES = {}  # the same by a tensor's dtype, as they are met
+
+
+class _Types(set):
+    """Element types by name; it holds tensors' dtypes of these names, as they are met."""
+
+    def __init__(self, *names):
+        super().__init__()
+        self.names = names
+
+
+_IDS, _F32, _BYTES, _CODES = _Types("int32", "uint32"), _Types("float32"), _Types("uint8", "int8"), _Types("uint8", "int8", "int32", "uint32")
 
 
 def _dtype(x, given, name):
@@ -94,6 +97,50 @@ class B200Dispatch:
     def _check(self, rc: int):
         if rc != N.OK:
             raise N.B200Error(rc, self._lib.pssa_b200_last_error(self._h).decode())
+
+    # Addresses of device arrays as plain numbers, which ctypes passes as they are: a decode step's calls have a dozen of them and take
+    # 10 us. Raw addresses are taken as they are; of a tensor it is checked what would be read as something else or be no memory of
+    # this device, 0.2 us for each.
+    def _at(self, x, name, types):
+        """A dense array of one of `types`."""
+        if x is None:
+            return None
+        try:
+            if x.dtype in types and x.get_device() == self.device and x.is_contiguous():
+                return x.data_ptr()
+        except AttributeError:
+            pass
+        if not hasattr(x, "get_device"):
+            return self._address(x, name)
+        own = str(x.dtype).removeprefix("torch.")
+        if own in types.names and x.dtype not in types:
+            types.add(x.dtype)
+            return self._at(x, name, types)
+        raise TypeError(f"{name} must be a dense array of {' or '.join(types.names)} on device {self.device}: got "
+                        f"{'dense' if x.is_contiguous() else 'strided'} {own}, device {x.get_device()}")
+
+    def _typed(self, x, given, name, dense=False):
+        """An array whose type is its own or, of a raw address, `given`, and that type: rows of adjacent elements at any distance, or
+        (`dense`) adjacent ones."""
+        try:
+            if given is None and x.get_device() == self.device and (x.is_contiguous() or (not dense and x.stride(-1) == 1)):
+                return x.data_ptr(), _TORCH_DTYPES[x.dtype]
+        except (AttributeError, KeyError):
+            pass
+        kind = _dtype(x, given, name)
+        if not hasattr(x, "get_device"):
+            return self._address(x, name), kind
+        if x.get_device() == self.device and (x.is_contiguous() or (not dense and x.stride(-1) == 1)):
+            return x.data_ptr(), kind
+        raise TypeError(f"{name} must be {'a dense array' if dense else 'rows of adjacent elements'} on device {self.device}: got "
+                        f"{'dense' if x.is_contiguous() else 'strided'}, device {x.get_device()}")
+
+    def _address(self, x, name):
+        if x is None or isinstance(x, int):
+            return x
+        if not hasattr(x, "data_ptr"):
+            raise TypeError(f"{name} must be an array on device {self.device} or its address: got {type(x)}")
+        return x.data_ptr()  # another library's array
 
     # ---- context
     def set_stream(self, stream):
@@ -298,46 +345,62 @@ class B200Dispatch:
         """Log probability and rank of each row's target, entropy and the `top_n` best alternatives; only enqueues. `stats`
         [rows, 2] is what the gradient call takes back. `dtype` names the logits' type where they are a raw pointer. See
         pssa_b200_token_logprobs_dev in include/pssa_b200.h for masked rows and rows without a target."""
+        at = self._at
+        x, kind = self._typed(logits, dtype, "logits")
         self._check(self._lib.pssa_b200_token_logprobs_dev(
-            self._h, _addr(logits), _dtype(logits, dtype, "logits"), rows, vocab, vocab if ld is None else ld, temperature, _addr(targets),
-            _addr(logprob), _addr(rank), _addr(entropy), _addr(stats), top_n, _addr(top_ids), _addr(top_logprobs)))
+            self._h, x, kind, rows, vocab, vocab if ld is None else ld, temperature,
+            at(targets, "targets", _IDS), at(logprob, "logprob", _F32), at(rank, "rank", _IDS), at(entropy, "entropy", _F32),
+            at(stats, "stats", _F32), top_n, at(top_ids, "top_ids", _IDS), at(top_logprobs, "top_logprobs", _F32)))
 
     def token_logprobs_grad_dev(self, logits, rows, vocab, targets, stats, grad_logits, grad_logprob=None, entropy=None,
                                 grad_entropy=None, temperature=1.0, ld=None, ld_grad=None, dtype=None):
         """Gradient with respect to the logits of sum(grad_logprob * logprob + grad_entropy * entropy), with `stats` and `entropy`
         of the forward call; `grad_logits` has the logits' type and may be the logits themselves."""
-        if _dtype(grad_logits, dtype, "grad_logits") != _dtype(logits, dtype, "logits"):
+        at = self._at
+        x, kind = self._typed(logits, dtype, "logits")
+        grad, grad_kind = self._typed(grad_logits, dtype, "grad_logits")
+        if grad_kind != kind:
             raise TypeError("grad_logits must have the type of the logits")
         self._check(self._lib.pssa_b200_token_logprobs_grad_dev(
-            self._h, _addr(logits), _dtype(logits, dtype, "logits"), rows, vocab, vocab if ld is None else ld, temperature, _addr(targets),
-            _addr(stats), _addr(entropy), _addr(grad_logprob), _addr(grad_entropy), _addr(grad_logits), vocab if ld_grad is None else ld_grad))
+            self._h, x, kind, rows, vocab, vocab if ld is None else ld, temperature,
+            at(targets, "targets", _IDS), at(stats, "stats", _F32), at(entropy, "entropy", _F32), at(grad_logprob, "grad_logprob", _F32),
+            at(grad_entropy, "grad_entropy", _F32), grad, vocab if ld_grad is None else ld_grad))
 
     def distill_topk_dev(self, logits, rows, vocab, teacher_ids, teacher, k, kl=None, grad_kl=None, targets=None, ce=None, grad_ce=None,
                          grad_logits=None, temperature=1.0, teacher_temperature=1.0, rest=False, ld=None, ld_grad=None, dtype=None):
         """Divergence of the student from a teacher's `k` best ids (and a target's cross entropy) and, with `grad_logits`, the
         gradient of sum(grad_kl * kl + grad_ce * ce) in the same call. `teacher`: logits, or log probabilities whose missing mass
         belongs to all other ids (`rest=True`). See pssa_b200_distill_topk_dev in include/pssa_b200.h."""
-        if grad_logits is not None and _dtype(grad_logits, dtype, "grad_logits") != _dtype(logits, dtype, "logits"):
+        at = self._at
+        x, kind = self._typed(logits, dtype, "logits")
+        grad, grad_kind = (None, kind) if grad_logits is None else self._typed(grad_logits, dtype, "grad_logits")
+        if grad_kind != kind:
             raise TypeError("grad_logits must have the type of the logits")
         self._check(self._lib.pssa_b200_distill_topk_dev(
-            self._h, _addr(logits), _dtype(logits, dtype, "logits"), rows, vocab, vocab if ld is None else ld, temperature,
-            _addr(teacher_ids), _addr(teacher), k, teacher_temperature, _addr(targets), N.DISTILL_REST if rest else 0, _addr(kl), _addr(ce),
-            _addr(grad_kl), _addr(grad_ce), _addr(grad_logits), vocab if ld_grad is None else ld_grad))
+            self._h, x, kind, rows, vocab, vocab if ld is None else ld, temperature,
+            at(teacher_ids, "teacher_ids", _IDS), at(teacher, "teacher", _F32), k, teacher_temperature, at(targets, "targets", _IDS),
+            N.DISTILL_REST if rest else 0, at(kl, "kl", _F32), at(ce, "ce", _F32), at(grad_kl, "grad_kl", _F32), at(grad_ce, "grad_ce", _F32),
+            grad, vocab if ld_grad is None else ld_grad))
 
     # ---- products with 4-bit weights (device pointers)
     def w4_quantize_dev(self, w, n, k, group, codes, scales, zeros=None, dtype=None, scale_dtype=None):
         """The matrix w [n, k] as 4-bit codes [n, k/2] with a scale (and, with `zeros`, a zero) for each `group` of columns."""
-        self._check(self._lib.pssa_b200_w4_quantize_dev(self._h, _addr(w), _dtype(w, dtype, "w"), n, k, group, _addr(codes), _addr(scales),
-                                                        _dtype(scales, scale_dtype, "scales"), _addr(zeros)))
+        at = self._at
+        self._check(self._lib.pssa_b200_w4_quantize_dev(
+            self._h, *self._typed(w, dtype, "w", True), n, k, group, at(codes, "codes", _CODES), *self._typed(scales, scale_dtype, "scales", True),
+            at(zeros, "zeros", _BYTES)))
 
     def gemv_w4_dev(self, x, rows, codes, scales, zeros, n, k, group, out, ldx=None, ldo=None, epilogue=N.EPI_NONE, alpha=1.0,
                     dtype=None, scale_dtype=None):
         """out[rows, n] = epilogue(x[rows, k] * W[n, k]^T) with W in 4 bits, for the few rows of a decode step; only enqueues."""
-        if _dtype(out, dtype, "out") != _dtype(x, dtype, "x"):
+        at = self._at
+        vectors, kind = self._typed(x, dtype, "x")
+        result, result_kind = self._typed(out, dtype, "out")
+        if result_kind != kind:
             raise TypeError("out must have the type of x")
         self._check(self._lib.pssa_b200_gemv_w4_dev(
-            self._h, _addr(x), _dtype(x, dtype, "x"), rows, k if ldx is None else ldx, _addr(codes), _addr(scales),
-            _dtype(scales, scale_dtype, "scales"), _addr(zeros), n, k, group, _addr(out), n if ldo is None else ldo, epilogue, alpha))
+            self._h, vectors, kind, rows, k if ldx is None else ldx, at(codes, "codes", _CODES), *self._typed(scales, scale_dtype, "scales", True),
+            at(zeros, "zeros", _BYTES), n, k, group, result, n if ldo is None else ldo, epilogue, alpha))
 
     # ---- bank write / plastic fast weights (device pointers)
     def bank_insert_protected_dev(self, keys, norm_sq, values, confidence, last_seen_step, meta, capacity, d_key, d_val,
