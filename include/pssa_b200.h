@@ -616,8 +616,9 @@ int32_t pssa_b200_model_score(pssa_b200_model* m, uint32_t stream, const uint64_
  * pssa_b200_model_score with what pssa_b200_token_logprobs_dev gives for every position: log probability, rank and entropy of
  * the targets and the top_n best alternatives, at `temperature`. The carry advances like a prefill's. HOST pointers: ids [n],
  * targets [n] (NULL when neither logprob nor rank is wanted; UINT64_MAX: a position without a target), logprob, entropy [n], rank [n]
- * u32, top_ids u64 (UINT64_MAX behind the vocabulary's end) and top_logprobs [n, top_n]; outputs may be NULL. Non-finite logits
- * are an error, as in the scorer; outputs then hold the positions before the pass that failed.
+ * u32, top_ids u64 (UINT64_MAX behind the vocabulary's end) and top_logprobs [n, top_n]; outputs may be NULL. As in the scorer it
+ * is an error when a position's logits hold a NaN, +inf or nothing above -inf, or its target has no finite log probability;
+ * outputs then hold the positions before the pass that failed.
  */
 int32_t pssa_b200_model_score_logprobs(pssa_b200_model* m, uint32_t stream, const uint64_t* ids, const uint64_t* targets, size_t n,
                                        float temperature, float* logprob, uint32_t* rank, float* entropy, size_t top_n, uint64_t* top_ids,

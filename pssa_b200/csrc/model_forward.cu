@@ -1018,8 +1018,8 @@ static int32_t score_answers(pssa_b200_model* m, uint32_t stream, const uint64_t
     auto& sc = m->score;
     int32_t rc = score_reserve(m, window, tile);
     if (rc) return rc;
-    // a pass's results, one array after another: log probability, entropy, rank, alternatives' ids, their log probabilities
-    const size_t words = window * (3 + 2 * top_n);
+    // a pass's results, one array after another: log probability, entropy, rank, statistics, alternatives' ids, their log probabilities
+    const size_t words = window * (5 + 2 * top_n);
     if (words * 4 > sc.answer_bytes) {
         PSSA_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
         cudaFree(sc.answers);
@@ -1043,24 +1043,31 @@ static int32_t score_answers(pssa_b200_model* m, uint32_t stream, const uint64_t
         float* lp = reinterpret_cast<float*>(sc.answers);
         float* ent = lp + rows;
         uint32_t* rk = reinterpret_cast<uint32_t*>(ent + rows);
-        uint32_t* tid = rk + rows;
+        float* stats = reinterpret_cast<float*>(rk + rows);
+        uint32_t* tid = rk + 3 * rows;
         float* tlp = reinterpret_cast<float*>(tid + rows * top_n);
         for (size_t r0 = 0; r0 < rows; r0 += tile) {
             const size_t nr = std::min(tile, rows - r0);
             if ((rc = score_logits(m, feats + r0 * m->d, nr))) return rc;
             LogprobParams p{};
             p.logits = sc.logits, p.dtype = PSSA_B200_F32, p.rows = nr, p.ld = m->v, p.vocab = (int)m->v, p.temperature = temperature;
-            p.targets = sc.targets + r0, p.logprob = lp + r0, p.rank = rk + r0, p.entropy = ent + r0, p.top_n = (int)top_n;
+            p.targets = sc.targets + r0, p.logprob = lp + r0, p.rank = rk + r0, p.entropy = ent + r0, p.stats = stats + 2 * r0, p.top_n = (int)top_n;
             p.top_ids = top_n ? tid + r0 * top_n : nullptr, p.top_logprobs = top_n ? tlp + r0 * top_n : nullptr, p.status = ctx->status_dev;
             if ((rc = launch_token_logprobs(ctx, p))) return rc;
         }
-        PSSA_CUDA(ctx, cudaMemcpyAsync(back.data(), sc.answers, rows * (3 + 2 * top_n) * 4, cudaMemcpyDeviceToHost, ctx->stream));
+        PSSA_CUDA(ctx, cudaMemcpyAsync(back.data(), sc.answers, rows * (5 + 2 * top_n) * 4, cudaMemcpyDeviceToHost, ctx->stream));
         PSSA_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
         const float* b_lp = reinterpret_cast<const float*>(back.data());
-        const uint32_t *b_rk = back.data() + 2 * rows, *b_ids = b_rk + rows;
+        const float* b_stats = b_lp + 3 * rows;
+        const uint32_t *b_rk = back.data() + 2 * rows, *b_ids = back.data() + 5 * rows;
         const float* b_tlp = reinterpret_cast<const float*>(b_ids + rows * top_n);
-        for (size_t t = 0; t < rows; ++t)
-            if (!std::isfinite(b_lp[rows + t])) return fail(ctx, PSSA_B200_ERR_INVALID_ARGUMENT, "model emitted non-finite logits at token %zu", t0 + t);
+        for (size_t t = 0; t < rows; ++t) {  // the scorer's loss would be none
+            if (!std::isfinite(b_stats[2 * t]))
+                return fail(ctx, PSSA_B200_ERR_INVALID_ARGUMENT, "model emitted non-finite logits at token %zu", t0 + t);
+            if (!std::isfinite(b_lp[t]))
+                return fail(ctx, PSSA_B200_ERR_INVALID_ARGUMENT,
+                            "the target at token %zu has no finite log probability: non-finite logits, or too low a temperature", t0 + t);
+        }
         if (logprob) std::copy(b_lp, b_lp + rows, logprob + t0);
         if (entropy) std::copy(b_lp + rows, b_lp + 2 * rows, entropy + t0);
         if (rank) std::copy(b_rk, b_rk + rows, rank + t0);

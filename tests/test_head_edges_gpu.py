@@ -136,3 +136,69 @@ def test_a_row_that_is_sure_of_one_id_keeps_its_small_numbers(gpu, dtype, rows, 
                               *([("best", got["top"][r, 0], -l)] if top else [])):
             assert abs(float(a) - want) <= tol * abs(want) + 2.0 ** -149, (name, r, float(a), want)
         assert got["rank"][r] == 1
+
+
+def test_a_model_whose_logits_are_no_numbers():
+    """What the scorer refuses `score_logprobs` refuses too: a target's logit of -inf, and a position of nothing else. An id that is
+    not the target may be one, in both."""
+    import oracle as O
+    import pssa_b200
+    from helpers import fill_synthetic, upload
+    from pssa_b200 import model as M
+    gpu = pssa_b200.B200Dispatch(0)
+    v, d = 203, 32
+    om = fill_synthetic(O.Model.new(2, v, d, 16, 8, 16, tau_mem=0.1, seed=5), 5)
+    m = pssa_b200.PSSAModel(gpu, 2, v, d, 16, 8, 16, tau_mem=0.1, precision=1)
+    upload(om, m)
+    start = m.copy_recurrent_state_to(0)
+    head = np.random.default_rng(0).standard_normal((v, d)).astype(np.float32)
+
+    def with_head(u, f):
+        m.set_tensor(-1, M.UNEMBED, u)
+        m.copy_recurrent_state_from(start, 0)
+        return f()
+
+    probe = head.copy()
+    probe[:d] = np.eye(d, dtype=np.float32)
+    features = with_head(probe, lambda: m.score([1], [0], want_logits=True))[2][0, :d] * np.sqrt(d)  # a head's scale is 1 / sqrt(d)
+    assert np.abs(features).sum() > 1.01
+    lowest = np.finfo(np.float32).min * np.sign(features)  # products of one sign: their sum is beyond fp32's range
+    one = head.copy()
+    one[7] = lowest
+    _, loss, logits = with_head(one, lambda: m.score([1], [3], want_logits=True))
+    assert logits[0, 7] == -np.inf and np.isfinite(np.delete(logits[0], 7)).all()
+    for f in (lambda: m.score([1], [7]), lambda: m.score_logprobs([1], [7]), lambda: m.score_logprobs([1, 1], [3, 7], top=2)):
+        with pytest.raises(pssa_b200.B200Error):
+            with_head(one, f)
+    got = with_head(one, lambda: m.score_logprobs([1], [3], top=4))
+    w = P.logprobs(logits[0].astype(np.float64), 3, 1.0, 4)
+    assert got["rank"][0] == w["rank"] and np.array_equal(got["top_ids"][0], w["ids"]) and abs(got["logprob"][0] - w["logprob"]) <= w["tol"] + P.U * 40
+    none = np.tile(lowest, (v, 1))
+    for f in (lambda: m.score([1], [3]), lambda: m.score_logprobs([1], [3]), lambda: m.score_logprobs([1]), lambda: m.score_logprobs([1], [-1], top=3)):
+        with pytest.raises(pssa_b200.B200Error):
+            with_head(none, f)
+    m.close()
+    gpu.close()
+
+
+def test_a_text_whose_logits_take_two_tiles():
+    """256 rows of 131072 logits are a tile: positions behind it, with their targets and alternatives."""
+    import pssa_b200
+    gpu = pssa_b200.B200Dispatch(0)
+    v, n, top = 131072, 300, 5
+    m = pssa_b200.PSSAModel(gpu, 1, v, 32, 16, 8, 16, tau_mem=0.1)
+    m.init_random(3)
+    m.set_max_rows(n)
+    rng = np.random.default_rng(1)
+    ids, targets = rng.integers(0, v, n), rng.integers(0, v, n)
+    start = m.copy_recurrent_state_to(0)
+    _, _, logits = m.score(ids, targets, want_logits=True)
+    m.copy_recurrent_state_from(start, 0)
+    got = m.score_logprobs(ids, targets, top=top)
+    for r in (0, 1, 254, 255, 256, 257, 298, 299):
+        w = P.logprobs(logits[r].astype(np.float64), int(targets[r]), 1.0, top)
+        assert got["rank"][r] == w["rank"] and np.array_equal(got["top_ids"][r], w["ids"])
+        assert abs(got["logprob"][r] - w["logprob"]) <= w["tol"] + P.U * 100 and abs(got["entropy"][r] - w["entropy"]) <= w["tol_h"]
+        assert np.max(np.abs(got["top_logprobs"][r] - w["top"])) <= w["tol"] + P.U * 100
+    m.close()
+    gpu.close()
