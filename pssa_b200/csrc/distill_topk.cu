@@ -312,6 +312,7 @@ __global__ void __launch_bounds__(32 * (ROW_WARPS + 1)) distill_topk_kernel(Dist
             if (!tc::mbar_wait(&s_bar[i], 0)) {
                 if (lane == 0) atomicExch(p.status, PSSA_B200_ERR_TIMEOUT);
                 tc::mbar_wait(&s_bar[i], 0);  // no CTA leaves with its copy on the way, if a wait can help it
+                rest.sum = pair(kNan, kNan);  // the row's results are none, as of a row with a NaN
             }
             const int last = min((i + 1) * piece, vecs), share = (last - i * piece + kRowWarps - 1) / kRowWarps;
             const int lo = min(i * piece + warp * share, last), hi = min(lo + share, last);
