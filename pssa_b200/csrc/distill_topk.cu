@@ -92,14 +92,9 @@ __global__ void __launch_bounds__(kThreads) distill_topk_long_kernel(DistillPara
     if (tid < PSSA_B200_MAX_TEACHER) s_id[tid] = entry ? id : PSSA_B200_NO_TOKEN, s_t[tid] = t;
     __syncthreads();
     bool first = entry;
-    float t_at = 0.0f;
     if (entry) {
         atomicOr(&s_bits[id >> 5], 1u << (id & 31));
-        for (int j = 0; j < p.k; ++j)
-            if (s_id[j] == id) {
-                first = first && j >= tid;
-                t_at += s_t[j];
-            }
+        for (int j = 0; j < tid; ++j) first = first && s_id[j] != id;
     }
     __syncthreads();
     float mu = -FLT_MAX;  // of the ids that are not listed: their sum is relative to their own maximum

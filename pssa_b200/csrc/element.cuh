@@ -22,13 +22,6 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { retu
 template <>
 __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 
-// an array's element by its type, where that is not known to the compiler
-__device__ __forceinline__ float load_f32(const void* p, int dtype, size_t i) {
-    if (dtype == PSSA_B200_F32) return static_cast<const float*>(p)[i];
-    if (dtype == PSSA_B200_BF16) return to_f32(static_cast<const __nv_bfloat16*>(p)[i]);
-    return to_f32(static_cast<const __half*>(p)[i]);
-}
-
 inline size_t dtype_size(int dtype) { return dtype == PSSA_B200_F32 ? 4 : 2; }
 
 // f(T()) for the type that `dtype` names
