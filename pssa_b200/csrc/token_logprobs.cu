@@ -411,8 +411,10 @@ int32_t launch_token_logprobs(pssa_b200_ctx* ctx, const LogprobParams& p) {
     while (ctas < kMaxCtas && p.rows * ctas < (size_t)ctx->sm_count && vecs / (ctas * 2) >= 256) ctas *= 2;
     const bool few = p.rows * ctas <= (size_t)ctx->sm_count && vecs / ctas >= 2048;  // more threads, where few CTAs have long parts
     // small CTAs where there are enough short rows: more rows on their way, and fewer threads to join for each (8000 x 1000 bf16 with 5
-    // alternatives 73 -> 37 us, 4245 x 16384 fp16 with 20 77 -> 66; 800 x 32768 32 -> 37, 2000 x 65536 61 -> 64)
-    const bool small = ctas == 1 && vecs <= 4096 && p.rows > (size_t)ctx->sm_count * 8;
+    // alternatives 71 -> 37 us, 4245 x 16384 fp16 with 20 66 -> 53). Their 64 pairs read n / 64 of a long row again for n
+    // alternatives, nearly all of it for the most there may be (2048 x 16384 fp32 with 5, 20 and 64: 36, 45 and 129 us, with 256
+    // threads 36, 40 and 52; 4245 x 16384 fp16 with 32, 48 and 64: 62, 78 and 178, with 256 threads 70, 78 and 87)
+    const bool small = ctas == 1 && vecs <= 4096 && p.rows > (size_t)ctx->sm_count * 8 && p.top_n <= 48 && vecs * p.top_n <= 65536;
     if (p.rows * ctas > 0x7fffffffull) return fail(ctx, PSSA_B200_ERR_SHAPE, "B200 log probabilities: too many rows; refusing launch");
     const cudaError_t e = with_dtype(p.dtype, [&](auto t) {
         using T = decltype(t);

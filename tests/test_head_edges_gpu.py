@@ -202,3 +202,19 @@ def test_a_text_whose_logits_take_two_tiles():
         assert np.max(np.abs(got["top_logprobs"][r] - w["top"])) <= w["tol"] + P.U * 100
     m.close()
     gpu.close()
+
+
+@pytest.mark.parametrize("vocab,top", [(1000, 48), (1000, 49), (1000, 64), (5000, 52), (5003, 64), (16384, 16), (16384, 17)])
+def test_alternatives_of_many_rows_on_both_sides_of_the_choice(gpu, vocab, top):
+    """More rows than the GPU has CTAs: the best ids in order and their log probabilities, whichever CTA takes a row."""
+    from test_token_logprobs_gpu import check_forward, forward
+    import torch
+    rng = np.random.default_rng(top)
+    view, x = logits_of(rng, 24, vocab, "float32")
+    many = view.repeat(50, 1)
+    targets = rng.integers(0, vocab, 24).astype(np.uint32)
+    got = forward(gpu, many, vocab, np.tile(targets, 50), top, 1.0)
+    check_forward({k: v[:24] for k, v in got.items()}, x, targets, top, 1.0)
+    for k, v in got.items():
+        v = torch.from_numpy(v.view(np.int32)).view(50, -1)
+        assert bool((v == v[:1]).all()), k
