@@ -590,7 +590,8 @@ int32_t pssa_b200_token_logprobs_grad_dev(pssa_b200_ctx* ctx, const void* logits
  * pssa_b200_token_logprobs_dev gives as top_ids and top_logprobs fits), kl, ce [rows] (NULL to skip), grad_kl, grad_ce [rows]
  * (needed with grad_logits for the losses that are to be trained; NULL: zero), targets [rows] (needed by ce and grad_ce). An
  * id of PSSA_B200_NO_TOKEN is an absent entry or target: it counts nothing, and a row without entries has kl 0. An id that is
- * listed twice has the sum of its entries' mass. vocab is at most 1638400. Other ids outside the vocabulary raise
+ * listed twice has the sum of its entries' mass in the gradient, which is that of the joined list; kl sums t ln t entry by entry,
+ * and so is less by the entropy of the split than that of the joined list, and may be below 0. vocab is at most 1638400. Other ids outside the vocabulary raise
  * PSSA_B200_ERR_TOKEN in the status word and count as absent (ce NaN). ln p is held in fp32 and is -inf below its range.
  * Masked student logits (-inf) under a teacher's mass give kl = +inf and a finite gradient; a row of masked ids only gives kl
  * (where the teacher has mass) and ce +inf and a zero gradient. A row with a NaN or +inf gives NaN. A row whose gradient
