@@ -593,7 +593,8 @@ int32_t pssa_b200_token_logprobs_grad_dev(pssa_b200_ctx* ctx, const void* logits
  * listed twice has the sum of its entries' mass in the gradient, which is that of the joined list; kl sums t ln t entry by entry,
  * and so is less by the entropy of the split than that of the joined list, and may be below 0. vocab is at most 1638400. Other ids outside the vocabulary raise
  * PSSA_B200_ERR_TOKEN in the status word and count as absent (ce NaN). ln p is held in fp32 and is -inf below its range.
- * Masked student logits (-inf) under a teacher's mass give kl = +inf and a finite gradient; a row of masked ids only gives kl
+ * Masked student logits (-inf) under a teacher's mass give kl = +inf and a finite gradient, and so does a rest that no id is left
+ * for, unless it is what rounding leaves of a full list's mass (at most 2^-20), which counts nothing; a row of masked ids only gives kl
  * (where the teacher has mass) and ce +inf and a zero gradient. A row with a NaN or +inf gives NaN. A row whose gradient
  * weights are all zero gets a zero gradient whatever its logits hold. A teacher's entry that is NaN, or +inf at its temperature,
  * makes its row's kl NaN, and the gradient too where grad_kl is not zero; ce and its gradient do not depend on the teacher.

@@ -42,6 +42,15 @@ __device__ __forceinline__ T block_reduce(T v, T* scratch, F op) {
     return v;
 }
 
+// The rest's term of the divergence. Where no id has it (all are listed, or masked) the student gives it nothing and the term is
+// infinite, but for what the rounding of a full list leaves: an entry's fp32 log probability q is off by 2^-24 of |q| and of the log
+// sum that it was made with, so their masses by at most 2^-24 (entropy + 10), below 2^-20 for 256 entries.
+constexpr float kRounding = 0x1p-20f;
+__device__ __forceinline__ float rest_term(float r, bool none_left, float log_rest) {
+    if (!(r > 0.0f) || (none_left && r <= kRounding)) return 0.0f;
+    return none_left ? INFINITY : r * (logf(r) - log_rest);
+}
+
 // a teacher's entry at its temperature; one that is +inf is no number like a NaN
 __device__ __forceinline__ float teacher_entry(const DistillParams& p, size_t row, int i) {
     const float q = p.teacher[row * p.k + i] * (1.0f / p.teacher_temperature);
@@ -114,7 +123,7 @@ __global__ void __launch_bounds__(kThreads) distill_topk_long_kernel(DistillPara
     const float ls = logf(s), log_rest = to_m * inv_t + logf(su) - ls, p_rest = expf(log_rest);
     float term = t > 0.0f || t != t ? t * (log_t - (empty ? -INFINITY : z - ls)) : 0.0f;
     float kl = block_reduce(term, s_f, sum);
-    if (r > 0.0f) kl += r * (logf(r) - (empty || su == 0.0f ? -INFINITY : log_rest));
+    kl += rest_term(r, empty || su == 0.0f, log_rest);
     const float mass = block_reduce(t, s_f, sum) + r;
     const uint32_t tgt = p.targets ? p.targets[row] : PSSA_B200_NO_TOKEN;
     const bool has = tgt < (uint32_t)v, none = tgt == PSSA_B200_NO_TOKEN;
@@ -395,7 +404,7 @@ __global__ void __launch_bounds__(32 * (ROW_WARPS + 1)) distill_topk_kernel(Dist
             if (t > 0.0f || t != t) kl += t * (s_teacher.log_t[i] - (empty ? -INFINITY : z_of(s_teacher.x[i]) - ls));
         }
         kl = warp_sum(kl);
-        if (r > 0.0f) kl += r * (logf(r) - (empty || all.sum == 0.0f ? -INFINITY : log_rest));
+        kl += rest_term(r, empty || all.sum == 0.0f, log_rest);
         if (lane == 0) {
             if (p.kl) p.kl[row] = bad ? kNan : kl;
             if (p.ce) p.ce[row] = none ? 0.0f : bad || !has ? kNan : empty ? INFINITY : logf(s1) - (xt - m);

@@ -218,3 +218,54 @@ def test_alternatives_of_many_rows_on_both_sides_of_the_choice(gpu, vocab, top):
     for k, v in got.items():
         v = torch.from_numpy(v.view(np.int32)).view(50, -1)
         assert bool((v == v[:1]).all()), k
+
+
+@pytest.mark.parametrize("rows,vocab,allowed", [(40, 40, 40), (40, 64, 64), (24, 5003, 30), (6, 400003, 30)])
+@pytest.mark.parametrize("temperature", [1.0, 2.0])
+def test_a_teacher_that_lists_every_id_there_is(gpu, rows, vocab, allowed, temperature):
+    """All ids of a small vocabulary, or all that a mask leaves, as `token_logprobs_dev` gives them: what rounding leaves of the
+    teacher's mass belongs to no id, and is no infinite divergence. A mass that is left in earnest is one."""
+    import torch
+    from test_token_logprobs_gpu import forward
+    rng = np.random.default_rng(vocab)
+    x, y = rng.standard_normal((rows, vocab)) * 3, rng.standard_normal((rows, vocab)) * 3
+    masked = np.stack([rng.permutation(vocab) >= allowed for _ in range(rows)])
+    x[masked], y[masked] = -np.inf, -np.inf
+    teacher, student = (torch.from_numpy(a.astype(np.float32)).cuda() for a in (x, y))
+    x, y = teacher.double().cpu().numpy(), student.double().cpu().numpy()
+    top = min(vocab, 64)
+    got = forward(gpu, teacher, vocab, np.full(rows, P.NONE, np.uint32), top, 1.0)
+    g = np.ones(rows, np.float32)
+    kl, _, grad = distill(gpu, student, got["ids"], got["top"], None, g, None, temperature, 1.0, True)
+    grad = grad.double().cpu().numpy()
+    for r in range(rows):
+        zt, lt = P.log_softmax(x[r], 1.0)
+        zs, ls = P.log_softmax(y[r], temperature)
+        live = ~masked[r]
+        t = np.exp(zt[live] - lt)
+        want = float((t * (zt[live] - lt - zs[live] + ls)).sum())
+        # the entries' rounding, and the statistics' of both rows: of numbers of this size
+        size = float((t * (np.abs(zt[live] - lt) + np.abs(zs[live] - ls))).sum()) + abs(ls) + 1
+        tol = P.U * (2 * P.adds(vocab) + 60) * size
+        assert abs(kl[r] - want) <= tol, (r, kl[r], want)
+        d = np.zeros(vocab)
+        d[live] = (np.exp(zs[live] - ls) - t) / temperature
+        assert np.abs(grad[r] - d).max() <= P.U * (2 * P.adds(vocab) + 60) * (1 + np.abs(zs[live]).max()), r
+    less = got["top"] - np.float32(0.01)  # 1 % of the mass is left, and no id for it
+    kl, _, _ = distill(gpu, student, got["ids"], less, None, None, None, temperature, 1.0, True, grad=False)
+    assert np.isposinf(kl).all()
+
+
+@pytest.mark.parametrize("dtype,vocab", [("float32", 393216), ("float32", 393215), ("bfloat16", 786432), ("float32", 393217), ("bfloat16", 786433), ("float16", 1638400)])
+def test_distillation_on_both_sides_of_what_a_cluster_holds(gpu, dtype, vocab):
+    import pssa_b200
+    from test_distill_gpu import check, teacher_of
+    rng = np.random.default_rng(vocab)
+    view, x = logits_of(rng, 2, vocab, dtype, 1, vocab + 1)
+    ids, teacher = teacher_of(rng, x, 30, True)
+    targets, g = np.array([vocab - 1, 5], np.uint32), np.array([1.0, -0.5], np.float32)
+    check(distill(gpu, view, ids, teacher, targets, g, g, 2.0, 1.0, True), x, ids, teacher, targets, g, g, 2.0, 1.0, True, dtype)
+    if vocab == 1638400:
+        wide = view.new_zeros(2, vocab + 1)
+        with pytest.raises(pssa_b200.B200Error):
+            gpu.distill_topk_dev(wide, 2, vocab + 1, dev(ids), dev(teacher), 30, kl=dev(np.zeros(2, np.float32)), rest=True)
