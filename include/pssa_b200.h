@@ -554,7 +554,7 @@ int32_t pssa_b200_sample_dev(pssa_b200_ctx* ctx, float* logits, float* probs, si
  * entropy [rows], stats [rows, 2], rank [rows] u32; each output may be NULL. top_n <= PSSA_B200_MAX_TOP. Logits of -inf are
  * masked ids: probability 0, log probability -inf. A row of nothing else has logprob -inf, entropy 0, stats {-inf, 0}, rank 1.
  * A row that holds a NaN or +inf has no distribution: its fp32 results are NaN, rank 0, top_ids PSSA_B200_NO_TOKEN. A row's
- * bits do not depend on the other rows, but may on their number. Arrays of u32 and fp32 are dense and start on 4 bytes, in this call
+ * bits do not depend on the other rows, but may on their number and on where it starts. Arrays of u32 and fp32 are dense and start on 4 bytes, in this call
  * and the two below.
  */
 int32_t pssa_b200_token_logprobs_dev(pssa_b200_ctx* ctx, const void* logits, int32_t dtype, size_t rows, size_t vocab, size_t ld,

@@ -44,26 +44,33 @@ bool words(std::initializer_list<const void*> arrays) {
     return true;
 }
 
-// [rows, cols] elements with a row pitch: its extent in bytes
-int32_t pitched(pssa_b200_ctx* ctx, const char* what, const char* array, size_t rows, size_t cols, size_t ld, int32_t dtype, const void* p, size_t* bytes) {
+// [rows, cols] elements with a row pitch, in bytes
+struct Pitched {
+    uintptr_t start;
+    size_t bytes, width, pitch;  // from the first element to behind the last; of a row; from row to row
+};
+int32_t pitched(pssa_b200_ctx* ctx, const char* what, const char* array, size_t rows, size_t cols, size_t ld, int32_t dtype, const void* p, Pitched* out) {
     if (ld < cols) return fail(ctx, PSSA_B200_ERR_SHAPE, "B200 %s: pitch %zu of %s is smaller than its width %zu; refusing launch", what, ld, array, cols);
     int32_t rc;
     size_t n;
     if ((rc = f32_elems(ctx, what, {rows, ld}, &n))) return rc;
     const size_t size = dtype_size(dtype);
     if (!aligned(p, size)) return fail(ctx, PSSA_B200_ERR_INVALID_ARGUMENT, "B200 %s: %s is not aligned to its element; refusing launch", what, array);
-    *bytes = ((rows - 1) * ld + cols) * size;
+    *out = Pitched{reinterpret_cast<uintptr_t>(p), ((rows - 1) * ld + cols) * size, cols * size, ld * size};
     return PSSA_B200_OK;
 }
 
-bool overlap(const void* a, size_t na, const void* b, size_t nb) {
-    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-    return x < y + nb && y < x + na;
+// whether two arrays share an element: not where the rows of one lie between those of the other, at the same pitch
+bool overlap(const Pitched& a, const Pitched& b) {
+    if (a.start >= b.start + b.bytes || b.start >= a.start + a.bytes) return false;
+    if (a.pitch != b.pitch) return true;
+    const size_t off = b.start >= a.start ? (b.start - a.start) % a.pitch : a.pitch - 1 - (a.start - b.start - 1) % a.pitch;  // of b's rows in a's
+    return off < a.width || off + b.width > a.pitch;
 }
 
 // rows of logits and the temperature they are read at
 int32_t logits_shape(pssa_b200_ctx* ctx, const char* what, const void* logits, int32_t dtype, size_t rows, size_t vocab, size_t ld, float temperature,
-                     size_t* bytes) {
+                     Pitched* extent) {
     if (!logits) return invalid(ctx, what, "null logits");
     if (!known_dtype(dtype)) return fail(ctx, PSSA_B200_ERR_INVALID_ARGUMENT, "B200 %s: unknown element type %d; refusing launch", what, dtype);
     if (rows == 0 || vocab == 0 || rows > 0x7fffffff || vocab > 0x7fffffff)
@@ -71,16 +78,15 @@ int32_t logits_shape(pssa_b200_ctx* ctx, const char* what, const void* logits, i
     // 1 / T, and the same for powers of two, have to be numbers
     if (!(temperature > 0.0f) || !std::isfinite(temperature) || !std::isfinite(1.4427f / temperature))
         return fail(ctx, PSSA_B200_ERR_INVALID_ARGUMENT, "B200 %s: temperature %g is not a positive finite number; refusing launch", what, (double)temperature);
-    return pitched(ctx, what, "the logits", rows, vocab, ld, dtype, logits, bytes);
+    return pitched(ctx, what, "the logits", rows, vocab, ld, dtype, logits, extent);
 }
 
 // a gradient may lie in the logits' own place, or clear of them
-int32_t gradient_place(pssa_b200_ctx* ctx, const char* what, const void* logits, size_t bytes, size_t ld, void* grad, size_t ld_grad, size_t rows,
-                       size_t vocab, int32_t dtype) {
-    size_t n;
-    const int32_t rc = pitched(ctx, what, "the gradient", rows, vocab, ld_grad, dtype, grad, &n);
+int32_t gradient_place(pssa_b200_ctx* ctx, const char* what, const Pitched& logits, void* grad, size_t ld_grad, size_t rows, size_t vocab, int32_t dtype) {
+    Pitched g;
+    const int32_t rc = pitched(ctx, what, "the gradient", rows, vocab, ld_grad, dtype, grad, &g);
     if (rc) return rc;
-    if (grad == logits ? rows > 1 && ld != ld_grad : overlap(logits, bytes, grad, n))
+    if (g.start == logits.start ? rows > 1 && g.pitch != logits.pitch : overlap(logits, g))
         return invalid(ctx, what, "the gradient overlaps the logits without lying in their place");
     return PSSA_B200_OK;
 }
@@ -136,10 +142,10 @@ int32_t pssa_b200_gemv_w4_dev(pssa_b200_ctx* ctx, const void* x, int32_t dtype, 
     if (rows == 0 || rows > 0x7fffffff) return fail(ctx, PSSA_B200_ERR_SHAPE, "B200 %s: row count must be in 1..2^31-1; refusing launch", what);
     if (epilogue < PSSA_B200_EPI_NONE || epilogue > PSSA_B200_EPI_ADD_OUT)
         return fail(ctx, PSSA_B200_ERR_INVALID_ARGUMENT, "B200 %s: unknown epilogue %d; refusing launch", what, epilogue);
-    size_t nx, no;
-    if ((rc = pitched(ctx, what, "x", rows, k, ldx, dtype, x, &nx))) return rc;
-    if ((rc = pitched(ctx, what, "out", rows, n, ldo, dtype, out, &no))) return rc;
-    if (overlap(x, nx, out, no)) return invalid(ctx, what, "x and out overlap");
+    Pitched from, to;
+    if ((rc = pitched(ctx, what, "x", rows, k, ldx, dtype, x, &from))) return rc;
+    if ((rc = pitched(ctx, what, "out", rows, n, ldo, dtype, out, &to))) return rc;
+    if (overlap(from, to)) return invalid(ctx, what, "x and out overlap");
     const OnDevice on(ctx->device);
     PSSA_CUDA(ctx, on.error);
     GemvW4Params p{};
@@ -153,8 +159,8 @@ int32_t pssa_b200_token_logprobs_dev(pssa_b200_ctx* ctx, const void* logits, int
                                      uint32_t* top_ids, float* top_logprobs) {
     if (!ctx) return fail(nullptr, PSSA_B200_ERR_INVALID_ARGUMENT, "null context");
     const char* what = "log probabilities";
-    size_t bytes;
-    const int32_t rc = logits_shape(ctx, what, logits, dtype, rows, vocab, ld, temperature, &bytes);
+    Pitched extent;
+    const int32_t rc = logits_shape(ctx, what, logits, dtype, rows, vocab, ld, temperature, &extent);
     if (rc) return rc;
     if (top_n > PSSA_B200_MAX_TOP)
         return fail(ctx, PSSA_B200_ERR_UNSUPPORTED, "B200 %s: %zu alternatives are more than %d; refusing launch", what, top_n, PSSA_B200_MAX_TOP);
@@ -177,14 +183,14 @@ int32_t pssa_b200_token_logprobs_grad_dev(pssa_b200_ctx* ctx, const void* logits
                                           const float* grad_entropy, void* grad_logits, size_t ld_grad) {
     if (!ctx) return fail(nullptr, PSSA_B200_ERR_INVALID_ARGUMENT, "null context");
     const char* what = "log probabilities' gradient";
-    size_t bytes;
-    int32_t rc = logits_shape(ctx, what, logits, dtype, rows, vocab, ld, temperature, &bytes);
+    Pitched extent;
+    int32_t rc = logits_shape(ctx, what, logits, dtype, rows, vocab, ld, temperature, &extent);
     if (rc) return rc;
     if (!grad_logits || !stats) return invalid(ctx, what, "null gradient or stats");
     if (grad_logprob && !targets) return invalid(ctx, what, "a weight of the log probability needs targets");
     if (grad_entropy && !entropy) return invalid(ctx, what, "a weight of the entropy needs the entropy");
     if (!words({targets, stats, entropy, grad_logprob, grad_entropy})) return invalid(ctx, what, "an array is not aligned to its elements");
-    if ((rc = gradient_place(ctx, what, logits, bytes, ld, grad_logits, ld_grad, rows, vocab, dtype))) return rc;
+    if ((rc = gradient_place(ctx, what, extent, grad_logits, ld_grad, rows, vocab, dtype))) return rc;
     const OnDevice on(ctx->device);
     PSSA_CUDA(ctx, on.error);
     LogprobGradParams p{};
@@ -200,8 +206,8 @@ int32_t pssa_b200_distill_topk_dev(pssa_b200_ctx* ctx, const void* logits, int32
                                    size_t ld_grad) {
     if (!ctx) return fail(nullptr, PSSA_B200_ERR_INVALID_ARGUMENT, "null context");
     const char* what = "distillation";
-    size_t bytes;
-    int32_t rc = logits_shape(ctx, what, logits, dtype, rows, vocab, ld, temperature, &bytes);
+    Pitched extent;
+    int32_t rc = logits_shape(ctx, what, logits, dtype, rows, vocab, ld, temperature, &extent);
     if (rc) return rc;
     if (!teacher_ids || !teacher) return invalid(ctx, what, "null teacher");
     if (k == 0) return fail(ctx, PSSA_B200_ERR_SHAPE, "B200 %s: a teacher has at least one entry for a row; refusing launch", what);
@@ -218,7 +224,7 @@ int32_t pssa_b200_distill_topk_dev(pssa_b200_ctx* ctx, const void* logits, int32
     if (!grad_logits && (grad_kl || grad_ce)) return invalid(ctx, what, "weights of losses without a gradient");
     if (!kl && !ce && !grad_logits) return invalid(ctx, what, "no output is asked for");
     if (!words({teacher_ids, teacher, targets, kl, ce, grad_kl, grad_ce})) return invalid(ctx, what, "an array is not aligned to its elements");
-    if (grad_logits && (rc = gradient_place(ctx, what, logits, bytes, ld, grad_logits, ld_grad, rows, vocab, dtype))) return rc;
+    if (grad_logits && (rc = gradient_place(ctx, what, extent, grad_logits, ld_grad, rows, vocab, dtype))) return rc;
     const OnDevice on(ctx->device);
     PSSA_CUDA(ctx, on.error);
     DistillParams p{};

@@ -32,6 +32,22 @@ def test_arrays_of_words_start_on_words(tmp_path):
                "CALL(W, OK, c.z += 1); CALL(V, OK, c.z += 3); CALL(L, OK, c.tgt += 4); CALL(D, OK, c.te += 4);")
 
 
+
+def test_rows_may_lie_between_each_other(tmp_path):
+    """Two arrays with the same pitch in bytes whose rows alternate share no element; anything less is refused."""
+    run_checks(tmp_path, "".join(f"""
+CALL({c}, OK, (c.ld = 2000, c.ldg = 2000, c.g = c.x + 4000)); CALL({c}, OK, (c.ld = 2000, c.ldg = 2000, c.g = c.x - 4000));
+CALL({c}, ARG, (c.ld = 2000, c.ldg = 2000, c.g = c.x + 3996)); CALL({c}, ARG, (c.ld = 2000, c.ldg = 2000, c.g = c.x + 4004));
+CALL({c}, OK, (c.ld = 2001, c.ldg = 2001, c.g = c.x + 4004)); CALL({c}, OK, (c.ld = 2001, c.ldg = 2001, c.g = c.x + 8004 + 4000));
+CALL({c}, ARG, (c.ld = 1999, c.ldg = 1999, c.g = c.x + 4000)); CALL({c}, ARG, (c.ld = 2000, c.ldg = 2001, c.g = c.x + 4000));
+CALL({c}, OK, (c.dtype = 1, c.ld = 2000, c.ldg = 2000, c.g = c.x + 2000));
+""" for c in "GD") + """
+CALL(V, OK, (c.ldx = 320, c.ldo = 320, c.out = c.x + 1024)); CALL(V, ARG, (c.ldx = 320, c.ldo = 320, c.out = c.x + 1020));
+CALL(V, ARG, (c.ldx = 320, c.ldo = 320, c.out = c.x + 1028)); CALL(V, ARG, (c.ldx = 319, c.ldo = 319, c.out = c.x + 1024));
+CALL(V, OK, (c.ldx = 320, c.ldo = 320, c.out = c.x - 256)); CALL(V, ARG, (c.ldx = 320, c.ldo = 64, c.out = c.x + 1024));
+""")
+
+
 class Array:
     """What the methods look at of a tensor."""
 

@@ -269,3 +269,33 @@ def test_distillation_on_both_sides_of_what_a_cluster_holds(gpu, dtype, vocab):
         wide = view.new_zeros(2, vocab + 1)
         with pytest.raises(pssa_b200.B200Error):
             gpu.distill_topk_dev(wide, 2, vocab + 1, dev(ids), dev(teacher), 30, kl=dev(np.zeros(2, np.float32)), rest=True)
+
+
+def test_rows_that_lie_between_each_other(gpu):
+    """Logits and their gradient, inputs and results side by side in the rows of one buffer, as the same calls with an array of its own for the
+    result (a row's bits may depend on how it is aligned)."""
+    import torch
+    rng = np.random.default_rng(2)
+    view, x = logits_of(rng, 24, 1000, "float32")
+    wide = torch.full((24, 2003), 8.0, device="cuda")
+    left, right = wide[:, :1000], wide[:, 1002:2002]
+    left.copy_(view)
+    g, ids, teacher = np.ones(24, np.float32), np.tile(np.array([[5, 9, 700]], np.uint32), (24, 1)), np.log(np.full((24, 3), 0.3, np.float32))
+    apart = distill(gpu, left, ids, teacher, None, g, None, 1.0, 1.0, True)
+    beside = distill(gpu, left, ids, teacher, None, g, None, 1.0, 1.0, True, out=right)
+    assert np.array_equal(apart[0], beside[0], equal_nan=True) and torch.equal(apart[2].nan_to_num(3.0), right.nan_to_num(3.0))
+    assert torch.equal(left, view) and bool((wide[:, 1000:1002] == 8.0).all()) and bool((wide[:, 2002:] == 8.0).all())
+    stats, targets = torch.zeros(24, 2, device="cuda"), dev(np.arange(24, dtype=np.uint32))
+    gpu.token_logprobs_dev(left, 24, 1000, stats=stats, ld=2003)
+    out = torch.zeros(24, 1000, device="cuda")
+    gpu.token_logprobs_grad_dev(left, 24, 1000, targets, stats, out, grad_logprob=dev(g), ld=2003)
+    gpu.token_logprobs_grad_dev(left, 24, 1000, targets, stats, right, grad_logprob=dev(g), ld=2003, ld_grad=2003)
+    assert torch.equal(out.nan_to_num(3.0), right.nan_to_num(3.0)) and torch.equal(left, view)
+    codes, scales = torch.randint(0, 256, (96, 128), dtype=torch.uint8, device="cuda"), torch.rand(96, 4, device="cuda")
+    both = torch.randn(5, 360, device="cuda")
+    before, x, y = both.clone(), both[:, :256], both[:, 260:356]
+    out = torch.zeros(5, 96, device="cuda")
+    gpu.gemv_w4_dev(before[:, :256].contiguous(), 5, codes, scales, None, 96, 256, 64, out)
+    gpu.gemv_w4_dev(x, 5, codes, scales, None, 96, 256, 64, y, ldx=360, ldo=360)
+    y_is, both[:, 260:356] = y.clone(), before[:, 260:356]
+    assert torch.equal(out, y_is) and torch.equal(both, before)
