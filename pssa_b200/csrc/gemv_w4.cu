@@ -28,9 +28,10 @@ constexpr int kThreads = 256;
 // registers of two columns 4 apart, by a mask and the bits of 128 (fp16: 1024) that put a code into a mantissa; x is staged with
 // its runs in that order.
 //
-// What bounds it: one row of 32768 x 8192 takes 40 us, 3.4 TB/s, of which 38 stay when all loads hit the same chunk: the 11
-// instructions that make 8 codes into numbers, at 16 warps an SM. 48 rows of 16384 x 4096 take 43 us: staging 11, joining and
-// storing 11, products and conversions the rest, one after another since every SM has one or two CTAs in step. Codes through a
+// What it spends: one row of 32768 x 8192 takes 40 us, 3.4 TB/s, of which 38 stay when all loads hit the same chunk. It issues in 55 %
+// of its slots: the conversion of the codes is most of the instructions, but the 16 warps of an SM also wait, with one chunk each
+// on its way, and 256 CTAs over 148 SMs leave 40 SMs half empty. 48 rows of 16384 x 4096 take 43 us: staging 11, joining and storing
+// 11, products and conversions the rest, one after another, with no pipe above 28 %. Codes through a
 // ring of bulk copies (73 us: a barrier and a trip for the scales per piece) and one tile of rows a warp with three chunks on
 // their way (58 us: the work per chunk beside the conversion, twice as often) were slower.
 constexpr int kWarps = kThreads / 32;

@@ -2,15 +2,19 @@
 //
 // Forward: one read of the row. Every thread keeps the running maximum, sum exp and sum exp * z of its vectors, counts the logits
 // above the target's, and remembers the vector of its maximum; the threads' and then the CTAs' numbers are joined in a fixed order.
+// One logit equal to the row's maximum stays out of the sums all the way, and ln sum exp z is log1p of the rest: a row that is sure
+// of one id has small numbers, and they keep their digits (0.1 to 0.3 us of a small call, 2 to 8 % of many short rows).
 // A few rows are split over the CTAs of a cluster, which meet in distributed shared memory: one launch and no workspace whatever
-// the shape. 4096 x 131072 bf16: 212 us, 5.1 TB/s, bound by 83 instructions for 8 logits at 75 % of the issue slots. One row of 16384:
-// 9 us, of which the launch of the cluster, two dependent trips for the target's logit and the choice of 20 alternatives.
+// the shape. Times are the kernel's in a graph of launches. 4096 x 131072 bf16: 207 us, 5.2 TB/s, at 84 instructions for 8 logits and
+// 77 % of the issue slots; 4096 x 65536 fp32, half the instructions a byte: 173 us, 6.2 TB/s, HBM. One row of 16384: 9.2 us, of
+// which the launch of the cluster, two dependent trips for the target's logit and the choice of 20 alternatives.
 //
-// Alternatives come from the same pass. The n-th best of the threads' maxima (of pairs of neighbouring threads) bounds the n-th
-// best logit from below, and no logit above the bound lies outside the n pairs that reach it: only their shares, n / pairs of the
-// row, are read again, and what is not below the bound, hardly more than n logits, is sorted. Keys are (value, lower id first) and so
-// never equal: ties change nothing. Where more pass than there is room for (logits in an order made for it), the n are drawn one by
-// one instead.
+// Alternatives come from the same pass. The n-th best of the maxima of pairs of neighbouring threads (64, 128 or 512 of them) bounds
+// the n-th best logit from below, and no logit above the bound lies outside the n pairs that reach it: only their shares, n / pairs
+// of the row, are read again, and what is not below the bound is ranked, each against each: hardly more than n logits where n is
+// well below the pairs, some n ln n where all pairs reach it, every logit where fewer pairs than n have one (8000 x 1000 bf16:
+// 5 alternatives 38 us, 48 54, 64 1360). Keys are (value, lower id first) and so never equal: ties change nothing. Where more pass
+// than there is room for (logits in an order made for it), the n are drawn one by one instead.
 //
 // Gradient: elementwise with the forward call's maximum and log sum, one read and one write: 4096 x 65536 bf16 in 159 us, 6.8 TB/s.
 #include <cooperative_groups.h>
