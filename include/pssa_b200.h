@@ -393,7 +393,8 @@ int32_t pssa_b200_w4_quantize_dev(pssa_b200_ctx* ctx, const void* w, int32_t dty
  * times input is exact: an fp32 input goes through as three bf16 pieces of its bits, as far down as bf16 reaches (2^-133). The
  * scale is applied to the fp32 sum of each group, or of each 128 columns of a longer one. A NaN among a row's inputs makes its
  * results NaN, an infinity makes them NaN or infinite, and no other row's. A row's bits do not depend on the other rows, but
- * may on their number. k is at most 8388480. out must not overlap the other arrays. Only enqueues; needs no workspace.
+ * may on their number. k is at most 8388480, rows at most 65535 * 48 (fp32: 65535 * 16). out must not overlap the other arrays.
+ * Only enqueues; needs no workspace.
  */
 int32_t pssa_b200_gemv_w4_dev(pssa_b200_ctx* ctx, const void* x, int32_t dtype, size_t rows, size_t ldx, const uint8_t* codes,
                               const void* scales, int32_t scale_dtype, const uint8_t* zeros, size_t n, size_t k, size_t group, void* out,
@@ -554,8 +555,8 @@ int32_t pssa_b200_sample_dev(pssa_b200_ctx* ctx, float* logits, float* probs, si
  * entropy [rows], stats [rows, 2], rank [rows] u32; each output may be NULL. top_n <= PSSA_B200_MAX_TOP. Logits of -inf are
  * masked ids: probability 0, log probability -inf. A row of nothing else has logprob -inf, entropy 0, stats {-inf, 0}, rank 1.
  * A row that holds a NaN or +inf has no distribution: its fp32 results are NaN, rank 0, top_ids PSSA_B200_NO_TOKEN. A row's
- * bits do not depend on the other rows, but may on their number and on where it starts. Arrays of u32 and fp32 are dense and start on 4 bytes, in this call
- * and the two below.
+ * bits do not depend on the other rows, but may on their number and on where it starts. Arrays of u32 and fp32 are dense and start
+ * on 4 bytes, in this call and the two below.
  */
 int32_t pssa_b200_token_logprobs_dev(pssa_b200_ctx* ctx, const void* logits, int32_t dtype, size_t rows, size_t vocab, size_t ld,
                                      float temperature, const uint32_t* targets, float* logprob, uint32_t* rank, float* entropy,
