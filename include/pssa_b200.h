@@ -599,6 +599,8 @@ int32_t pssa_b200_token_logprobs_grad_dev(pssa_b200_ctx* ctx, const void* logits
  * (where the teacher has mass) and ce +inf and a zero gradient. A row with a NaN or +inf gives NaN. A row whose gradient
  * weights are all zero gets a zero gradient whatever its logits hold. A teacher's entry that is NaN, or +inf at its temperature,
  * makes its row's kl NaN, and the gradient too where grad_kl is not zero; ce and its gradient do not depend on the teacher.
+ * kl and ce are fp32 differences of log probabilities: right to a few 2^-24 of those and of 1, not of themselves where they are
+ * small (pssa_b200_token_logprobs_dev's log probability of a target keeps its digits there).
  */
 int32_t pssa_b200_distill_topk_dev(pssa_b200_ctx* ctx, const void* logits, int32_t dtype, size_t rows, size_t vocab, size_t ld,
                                    float temperature, const uint32_t* teacher_ids, const float* teacher, size_t k,
